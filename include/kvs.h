@@ -329,6 +329,116 @@ int kvs_paged_fill_varlen_layers(uint32_t n_layers, const void *const *k_fills, 
                                  void *const *cache_vs, uint32_t num_blocks, uint32_t block_size,
                                  uint32_t *out_of_range, void *stream);
 
+/* ---- operators on a paged KV cache ----
+ * What a serving step computes on the caches that the fills above and the block calls write: the
+ * rows of new tokens (norm, rotation, fill), attention of one new token over the cache, and the
+ * eviction of tokens that attention hardly reads. No counterpart in the reference, whose model
+ * runtime is not part of the store.
+ *
+ * kvs_paged_cache describes one layer's cache: row (block, head, slot) of K is head_dim contiguous
+ * elements at k + block * k_strides[0] + head * k_strides[1] + slot * k_strides[2] (bytes, multiples
+ * of 16, as is the address; V likewise), which covers [num_blocks, heads, block_size, head_dim] and
+ * vLLM's [num_blocks, block_size, heads, head_dim]. page_table: [batch][max_blocks] int32; entries
+ * <= 0 hold nothing, entries >= num_blocks are out of range, and tokens in either take no part. An
+ * e4m3 cache holds value / k_scale and value / v_scale, saturated; other types use scales of 1.
+ * head_dim: a multiple of 8 (16 for e4m3) up to 256. Rows behind a request's length, and all that a
+ * masked slot holds, are not read. All arrays are device memory of one GPU; calls are asynchronous
+ * on `stream`, make no allocation and keep no state, so they can be captured into CUDA graphs. */
+#define KVS_DTYPE_BF16 0
+#define KVS_DTYPE_FP16 1
+#define KVS_DTYPE_E4M3 2
+typedef struct {
+  void *k, *v;
+  int64_t k_strides[3], v_strides[3];
+  const int32_t *page_table;
+  uint32_t num_blocks, n_heads, block_size, head_dim, batch, max_blocks;
+  int32_t dtype;
+  float k_scale, v_scale;
+} kvs_paged_cache;
+
+/* Norm, rotation and fill of new tokens. q, k, v: [n_tokens] rows of q_heads (or the cache's
+ * n_heads) heads, `*_strides` bytes between tokens and between heads (multiples of 16), of type
+ * `dtype` (bf16 or fp16: the cache's, unless that is e4m3). Per head of q and k:
+ * y = x * weight / sqrt(mean(x^2) + eps) where a weight [head_dim] of type `dtype` is given, then the
+ * rotation of the first `rotary` elements (a multiple of 8, up to head_dim) by the token's position:
+ * pairs (i, i + rotary / 2), or (2i, 2i + 1) with `interleaved`. cos_sin: [n_positions][rotary] fp32,
+ * the cosines of rotary / 2 frequencies, then their sines. The position is the token's cache
+ * position, or, with `positions` ([n_axes][n_tokens] int32, n_axes <= 32), one per axis, frequency i
+ * taking axis axes[i] ([rotary / 2] int32; null: axis 0; values outside are taken as the last axis).
+ * Computed in fp32 and rounded once. q goes to q_out (which may be q itself), k and v to the cache
+ * slots that kvs_paged_fill_varlen gives the tokens (cu_seqlens, start_positions). A token whose
+ * slot is out of range stores no k and v; one whose position is not in cos_sin stores neither and
+ * its q_out row is zero; each such token increments *out_of_range when given. Tokens behind the last
+ * sequence are left as they were, or their q_out rows zeroed with `zero_rest`. Two tokens of one
+ * call must not share a slot. */
+typedef struct {
+  const void *q, *k, *v;
+  void *q_out;
+  int64_t q_strides[2], k_strides[2], v_strides[2], q_out_strides[2];
+  const float *cos_sin;
+  const int32_t *cu_seqlens, *start_positions, *positions, *axes;
+  const void *q_weight, *k_weight;
+  uint32_t *out_of_range;
+  uint32_t n_tokens, q_heads, rotary, n_positions, n_axes;
+  int32_t dtype;
+  float eps;
+  int32_t interleaved, zero_rest;
+} kvs_qkv_rows;
+int kvs_qk_norm_rope_fill(const kvs_paged_cache *cache, const kvs_qkv_rows *rows, void *stream);
+
+/* Attention of one new token per request. q, out: [batch][q_heads] heads of head_dim elements of
+ * type `dtype` (bf16 or fp16: the cache's, unless that is e4m3), `*_strides` bytes between requests
+ * and between heads (multiples of 16); query head g reads KV head g / (q_heads / n_heads). Request b
+ * attends to its tokens [max(0, seq_lens[b] - window), seq_lens[b]) (window 0: all), seq_lens bounded
+ * by max_blocks * block_size: out = sum softmax(scale * q . k) v. A row with no token gives zeros and
+ * a log-sum-exp of -infinity. lse: optional [batch][q_heads] fp32, natural logarithm. weights_out
+ * (optional, [batch][n_heads][w_len] fp32, strides in elements between requests and heads, may be
+ * `weights`): weights_out[b][h][t] = weights[b][h][t] + the softmax weights of token t summed over the
+ * query heads of h, for t < seq_lens[b]; w_len must cover max_blocks * block_size. The order of every
+ * sum is fixed by the lengths, so equal calls give equal bits. workspace: at least
+ * kvs_decode_attention_workspace bytes, 256-byte aligned, its contents of no matter; concurrent
+ * calls need one each. */
+typedef struct {
+  const void *q;
+  void *out;
+  int64_t q_strides[2], out_strides[2];
+  const int32_t *seq_lens;
+  float *lse;
+  const float *weights;
+  float *weights_out;
+  int64_t weights_strides[2], weights_out_strides[2];
+  void *workspace;
+  uint64_t workspace_bytes;
+  uint32_t q_heads, window, w_len;
+  int32_t dtype;
+  float scale;
+} kvs_decode_rows;
+int kvs_decode_attention_workspace(const kvs_paged_cache *cache, const kvs_decode_rows *rows, int32_t device,
+                                   uint64_t *bytes);
+int kvs_paged_decode_attention(const kvs_paged_cache *cache, const kvs_decode_rows *rows, void *stream);
+
+/* Eviction by accumulated attention weight. Per request and KV head, of the tokens below
+ * seq_lens[b] that have a page: positions < first and >= seq_lens[b] - recent stay, and of the others
+ * those of the largest weight (equal weights: the lowest position; NaN counts as the largest), keep
+ * in all (first + recent <= keep). kept: [batch][n_heads][keep] int32, the kept positions in order,
+ * then -1; new_lens: [batch] int32, min(keep, tokens). Kept rows of K and V move to slots 0, 1, ... of
+ * dst_table ([batch][dst_blocks] int32, covering keep slots; its blocks must be in no other table row
+ * of the call), or, where dst_table is null, of the request's own blocks, in place (then shared by no
+ * other request). A slot without a valid block stores nothing and increments *out_of_range when
+ * given. weights: [batch][n_heads][w_len] fp32 (strides in elements between requests and heads), w_len
+ * covering max_blocks * block_size; weights_out (may be `weights`) receives the kept tokens' weights,
+ * then zeros up to seq_lens[b]. cache->dtype gives the element size only: rows are moved as they are. */
+typedef struct {
+  const int32_t *seq_lens, *dst_table;
+  const float *weights;
+  float *weights_out;
+  int64_t weights_strides[2], weights_out_strides[2];
+  int32_t *kept, *new_lens;
+  uint32_t *out_of_range;
+  uint32_t dst_blocks, w_len, wo_len, keep, first, recent;
+} kvs_evict_rows;
+int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *rows, void *stream);
+
 /* ---- chunk gather / scatter ops ----
  * gather_tp_shards_to_chip / pack_local_shards (patch 0003 gather.hpp lines 9372-9417) and
  * their inverses scatter_chunk_from_chip / unpack_local_shards (9418-9453).

@@ -69,6 +69,7 @@ def build(debug: bool = False, verbose: bool = False, force: bool = False) -> Pa
         return OUT
     flags = ARCH + [
         "-std=c++17",
+        "--threads", "0",  # compile the sources side by side
         "-lineinfo",
         "-O0" if debug else "-O3",
         "-Xcompiler", "-fPIC,-Wall,-Wno-unused-function",

@@ -1096,4 +1096,6 @@ cudaError_t launch_bucket_requests(const BucketParams &p, cudaStream_t stream) {
 
 uint64_t kernel_launches() { return g_launches.load(std::memory_order_relaxed); }
 
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
 }  // namespace kvs

@@ -147,6 +147,100 @@ class KernelTiming(C.Structure):
     _fields_ = [("launches", C.c_uint64), ("bytes", C.c_uint64), ("total_ms", C.c_double)]
 
 
+DTYPE_BF16, DTYPE_FP16, DTYPE_E4M3 = 0, 1, 2
+
+
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_strides", C.c_int64 * 3),
+        ("v_strides", C.c_int64 * 3),
+        ("page_table", C.c_void_p),
+        ("num_blocks", C.c_uint32),
+        ("n_heads", C.c_uint32),
+        ("block_size", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("batch", C.c_uint32),
+        ("max_blocks", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("k_scale", C.c_float),
+        ("v_scale", C.c_float),
+    ]
+
+
+class QkvRows(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("q_strides", C.c_int64 * 2),
+        ("k_strides", C.c_int64 * 2),
+        ("v_strides", C.c_int64 * 2),
+        ("q_out_strides", C.c_int64 * 2),
+        ("cos_sin", C.c_void_p),
+        ("cu_seqlens", C.c_void_p),
+        ("start_positions", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("axes", C.c_void_p),
+        ("q_weight", C.c_void_p),
+        ("k_weight", C.c_void_p),
+        ("out_of_range", C.c_void_p),
+        ("n_tokens", C.c_uint32),
+        ("q_heads", C.c_uint32),
+        ("rotary", C.c_uint32),
+        ("n_positions", C.c_uint32),
+        ("n_axes", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("eps", C.c_float),
+        ("interleaved", C.c_int32),
+        ("zero_rest", C.c_int32),
+    ]
+
+
+class DecodeRows(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("out", C.c_void_p),
+        ("q_strides", C.c_int64 * 2),
+        ("out_strides", C.c_int64 * 2),
+        ("seq_lens", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("weights_out", C.c_void_p),
+        ("weights_strides", C.c_int64 * 2),
+        ("weights_out_strides", C.c_int64 * 2),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+        ("q_heads", C.c_uint32),
+        ("window", C.c_uint32),
+        ("w_len", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class EvictRows(C.Structure):
+    _fields_ = [
+        ("seq_lens", C.c_void_p),
+        ("dst_table", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("weights_out", C.c_void_p),
+        ("weights_strides", C.c_int64 * 2),
+        ("weights_out_strides", C.c_int64 * 2),
+        ("kept", C.c_void_p),
+        ("new_lens", C.c_void_p),
+        ("out_of_range", C.c_void_p),
+        ("dst_blocks", C.c_uint32),
+        ("w_len", C.c_uint32),
+        ("wo_len", C.c_uint32),
+        ("keep", C.c_uint32),
+        ("first", C.c_uint32),
+        ("recent", C.c_uint32),
+    ]
+
+
 P = C.c_void_p
 _u8p = C.POINTER(C.c_uint8)
 _u32p = C.POINTER(C.c_uint32)
@@ -216,6 +310,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [C.c_uint32, C.POINTER(P), C.POINTER(P), C.c_uint32, C.c_uint32, C.c_uint32, P, C.c_uint32, P, C.c_uint32, P,
          C.POINTER(P), C.POINTER(P), C.c_uint32, C.c_uint32, P, P],
     ),
+    "kvs_qk_norm_rope_fill": (C.c_int, [C.POINTER(PagedCache), C.POINTER(QkvRows), P]),
+    "kvs_decode_attention_workspace": (C.c_int, [C.POINTER(PagedCache), C.POINTER(DecodeRows), C.c_int32, _u64p]),
+    "kvs_paged_decode_attention": (C.c_int, [C.POINTER(PagedCache), C.POINTER(DecodeRows), P]),
+    "kvs_evict_paged": (C.c_int, [C.POINTER(PagedCache), C.POINTER(EvictRows), P]),
     "kvs_client_set_timing": (C.c_int, [P, C.c_int]),
     "kvs_client_timing": (C.c_int, [P, C.POINTER(KernelTiming), C.POINTER(KernelTiming)]),
     "kvs_client_host_tier_timing": (C.c_int, [P, C.POINTER(KernelTiming), C.POINTER(KernelTiming)]),

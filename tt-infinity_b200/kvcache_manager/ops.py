@@ -1,5 +1,7 @@
-"""Chunk gather / scatter ops over paged KV members, and the token-granular paged fill (torch
-CUDA tensors).
+"""Chunk gather / scatter ops over paged KV members, the token-granular paged fill, and what a
+serving step computes on the paged caches: norm, rotation and fill of new tokens
+(`qk_norm_rope_fill`), attention of one new token per request (`paged_decode_attention`) and eviction
+by accumulated attention weight (`evict_paged_kv`). All take torch CUDA tensors.
 
 B200 counterparts of ttnn.kvcache_manager.gather_tp_shards_to_chip / scatter_chunk_from_chip /
 pack_local_shards / unpack_local_shards (patch 0003 gather.hpp lines 9335-9453). A "rank" is a
@@ -105,7 +107,9 @@ def unpack_local_shards(src: Any, members: Sequence[Any], block_ids: Sequence[in
     scatter_chunk_from_chip(src, [list(members)], block_ids, shard_block_bytes, region_bases, blocking)
 
 
-__all__ = ["gather_tp_shards_to_chip", "scatter_chunk_from_chip", "pack_local_shards", "unpack_local_shards"]
+__all__ = ["gather_tp_shards_to_chip", "scatter_chunk_from_chip", "pack_local_shards", "unpack_local_shards",
+           "paged_fill_cache_varlen", "paged_fill_cache_varlen_layers", "qk_norm_rope_fill",
+           "paged_decode_attention", "evict_paged_kv"]
 _ = _native
 
 
@@ -218,3 +222,291 @@ def paged_fill_cache_varlen_layers(k_fill_values: Sequence[Any], v_fill_values: 
         P(out_of_range.data_ptr() if out_of_range is not None else None),
         P(torch.cuda.current_stream(k0.device).cuda_stream)))
     return cache_ks, cache_vs
+
+
+# ---------------------------------------------------------------- operators on a paged cache
+
+
+def _dtype_code(dtype: Any) -> int:
+    torch = _torch()
+    return {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_FP16,
+            torch.float8_e4m3fn: _native.DTYPE_E4M3}.get(dtype, -1)
+
+
+def _on(device: Any, **tensors: Any) -> None:
+    """Every tensor given (None: not given) is a CUDA tensor on `device` that needs no gradient."""
+    torch = _torch()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+            raise RuntimeError(f"{name} must be on device!")
+        if t.device != device:
+            raise RuntimeError("All tensors must be on the same device!")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires grad, and the operators on a paged cache have no backward pass")
+
+
+def _int32(ndim: int, **tensors: Any) -> None:
+    torch = _torch()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.dtype != torch.int32:
+            raise RuntimeError(f"{name} must be INT32")
+        if t.dim() != ndim or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous, of {ndim} dimension(s)")
+
+
+def _strides(t: Any, n: int, unit: int) -> list[int]:
+    """Strides of the first n dimensions, `unit` bytes an element; a dimension of one element has none."""
+    return [unit * s if size > 1 else 0 for size, s in zip(t.shape[:n], t.stride())]
+
+
+def _rows(name: str, t: Any, ndim: int) -> None:
+    if t.dim() != ndim:
+        raise RuntimeError(f"{name} must be {ndim}-D")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise RuntimeError(f"{name} rows must be contiguous")
+
+
+def _paged_cache(cache_k: Any, cache_v: Any, page_table: Any, k_scale: float, v_scale: float):
+    """The C description of a layer's cache [num_blocks, num_kv_heads, block_size, head_dim], whose
+    first three dimensions may have any strides (vLLM's [num_blocks, block_size, heads, head_dim] is
+    passed as cache.transpose(1, 2))."""
+    torch = _torch()
+    if not isinstance(cache_k, torch.Tensor) or cache_k.device.type != "cuda":
+        raise RuntimeError("cache_k must be on device!")
+    _on(cache_k.device, cache_k=cache_k, cache_v=cache_v, page_table=page_table)
+    _rows("cache_k", cache_k, 4)
+    _rows("cache_v", cache_v, 4)
+    if cache_k.shape != cache_v.shape or cache_k.dtype != cache_v.dtype:
+        raise RuntimeError("cache_k and cache_v must have the same shape and dtype")
+    _int32(2, page_table=page_table)
+    code = _dtype_code(cache_k.dtype)
+    if code < 0:
+        raise RuntimeError(f"cache dtype ({cache_k.dtype}) must be bfloat16, float16 or float8_e4m3fn")
+    blocks, heads, size, dim = cache_k.shape
+    unit = cache_k.element_size()
+    S3 = C.c_int64 * 3
+    return _native.PagedCache(cache_k.data_ptr(), cache_v.data_ptr(), S3(*_strides(cache_k, 3, unit)),
+                              S3(*_strides(cache_v, 3, unit)), page_table.data_ptr(), blocks, heads, size, dim,
+                              page_table.shape[0], page_table.shape[1], code, k_scale, v_scale)
+
+
+def _stream(device: Any):
+    return C.c_void_p(_torch().cuda.current_stream(device).cuda_stream)
+
+
+def _check_counter(t: Any) -> None:
+    if t is not None and t.dtype != _torch().int32:
+        raise RuntimeError("out_of_range must be an int32 tensor")
+
+
+def _ptr(t: Any):
+    return None if t is None else t.data_ptr()
+
+
+_S2 = C.c_int64 * 2
+
+
+def qk_norm_rope_fill(q: Any, k: Any, v: Any, cos_sin: Any, cu_seqlens: Any, page_table: Any, start_positions: Any,
+                      cache_k: Any, cache_v: Any, *, q_weight: Any = None, k_weight: Any = None, eps: float = 1e-6,
+                      positions: Any = None, axes: Any = None, interleaved: bool = False, k_scale: float = 1.0,
+                      v_scale: float = 1.0, q_out: Any = None, out_of_range: Any = None):
+    """Per-head norms of queries and keys, rotation by the token's position and the fill of K and V
+    into a paged cache, in one pass over q, k and v. Returns (q_out, cache_k, cache_v).
+
+    q [tokens, q_heads, head_dim], k / v [tokens, num_kv_heads, head_dim]: bf16 or fp16, any strides
+    with contiguous rows on 16-byte boundaries (slices of one projection's output, for example).
+    cache_k / cache_v [num_blocks, num_kv_heads, block_size, head_dim] of the same dtype, or
+    float8_e4m3fn holding value / k_scale and value / v_scale, any strides with contiguous rows.
+    cu_seqlens, page_table and start_positions place the tokens as in paged_fill_cache_varlen.
+
+    Per head x of q and k: x * weight / sqrt(mean(x^2) + eps) where q_weight / k_weight ([head_dim],
+    the rows' dtype) is given, then the first cos_sin.shape[1] elements are rotated: pairs
+    (i, i + rotary / 2), or (2i, 2i + 1) with interleaved. cos_sin: fp32 [positions, rotary], cosines of
+    rotary / 2 frequencies, then their sines. A token's position is its position in the cache, or
+    comes from positions: int32 [tokens], or [n_axes, tokens] (time, height and width of an image's
+    tokens, say) with axes, int32 [rotary / 2], naming each frequency's axis. Computed in fp32 and
+    rounded once.
+
+    q_out may be q itself. A token whose slot is out of range stores no K and V; one whose position
+    is outside cos_sin stores neither and gets a zero q_out row; out_of_range (int32, one element)
+    counts both. Tokens behind the last sequence are left as they were in a given q_out and are zero
+    in one allocated here. Two tokens must not share a slot. Asynchronous on the current stream."""
+    torch = _torch()
+    cache = _paged_cache(cache_k, cache_v, page_table, k_scale, v_scale)
+    dev = cache_k.device
+    _on(dev, q=q, k=k, v=v, cos_sin=cos_sin, cu_seqlens=cu_seqlens, start_positions=start_positions,
+        q_weight=q_weight, k_weight=k_weight, positions=positions, axes=axes, q_out=q_out, out_of_range=out_of_range)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _rows(name, t, 3)
+    tokens, q_heads, dim = q.shape
+    if k.shape != v.shape or k.shape[0] != tokens or k.shape[1] != cache_k.shape[1]:
+        raise RuntimeError("k and v must be [tokens, num_kv_heads, head_dim], with q's tokens and the cache's heads")
+    if dim != cache_k.shape[3] or k.shape[2] != dim:
+        raise RuntimeError("head_dim of q, k and v must match the cache")
+    if not q.dtype == k.dtype == v.dtype:
+        raise RuntimeError("q, k and v must have the same dtype")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None and (t.shape != (dim,) or t.dtype != q.dtype or not t.is_contiguous()):
+            raise RuntimeError(f"{name} must be a contiguous [head_dim] tensor of q's dtype")
+    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous():
+        raise RuntimeError("cos_sin must be a contiguous float32 [positions, rotary] tensor")
+    _int32(1, cu_seqlens=cu_seqlens, start_positions=start_positions, axes=axes)
+    if start_positions.shape[0] != page_table.shape[0]:
+        raise RuntimeError(f"start_positions size ({start_positions.shape[0]}) must match batch_size ({page_table.shape[0]})")
+    if cu_seqlens.shape[0] != page_table.shape[0] + 1:
+        raise RuntimeError(f"cu_seqlens must hold batch_size + 1 = {page_table.shape[0] + 1} entries")
+    n_axes = 0
+    if positions is not None:
+        n_axes = positions.shape[0] if positions.dim() == 2 else 1
+        _int32(positions.dim(), positions=positions)
+        if positions.dim() not in (1, 2) or positions.shape[-1] != tokens:
+            raise RuntimeError("positions must be [tokens] or [n_axes, tokens]")
+    if axes is not None and axes.shape[0] * 2 != cos_sin.shape[1]:
+        raise RuntimeError("axes must hold rotary / 2 entries")
+    if axes is None and n_axes > 1:
+        raise RuntimeError("positions of several axes need axes")
+    _check_counter(out_of_range)
+    zero_rest = q_out is None
+    if q_out is None:
+        q_out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=dev)
+    else:
+        _rows("q_out", q_out, 3)
+        if q_out.shape != q.shape or q_out.dtype != q.dtype:
+            raise RuntimeError("q_out must have q's shape and dtype")
+    rows = _native.QkvRows(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), _S2(*_strides(q, 2, 2)), _S2(*_strides(k, 2, 2)),
+        _S2(*_strides(v, 2, 2)), _S2(*_strides(q_out, 2, 2)), cos_sin.data_ptr(), cu_seqlens.data_ptr(),
+        start_positions.data_ptr(), _ptr(positions), _ptr(axes), _ptr(q_weight), _ptr(k_weight), _ptr(out_of_range),
+        tokens, q_heads, cos_sin.shape[1], cos_sin.shape[0], n_axes, _dtype_code(q.dtype), eps, interleaved, zero_rest)
+    check(load().kvs_qk_norm_rope_fill(C.byref(cache), C.byref(rows), _stream(dev)))
+    return q_out, cache_k, cache_v
+
+
+def _weight_sums(name: str, t: Any, batch: int, heads: int, cover: int) -> None:
+    """A running sum of softmax weights: fp32 [batch, num_kv_heads, at least `cover` tokens]."""
+    torch = _torch()
+    if t.dtype != torch.float32 or t.dim() != 3 or t.stride(2) != 1 or t.shape[:2] != (batch, heads):
+        raise RuntimeError(f"{name} must be float32 [batch_size, num_kv_heads, tokens] with contiguous rows")
+    if t.shape[2] < cover:
+        raise RuntimeError(f"{name} must cover max_num_blocks_per_seq * block_size = {cover} tokens")
+
+
+def paged_decode_attention(q: Any, cache_k: Any, cache_v: Any, page_table: Any, seq_lens: Any, *,
+                           scale: float | None = None, window: int | None = None, k_scale: float = 1.0,
+                           v_scale: float = 1.0, out: Any = None, return_lse: bool = False, weights: Any = None,
+                           weights_out: Any = None):
+    """Attention of one new token per request over its paged K / V cache.
+
+    q [batch, q_heads, head_dim] (bf16 or fp16, any strides with contiguous rows on 16-byte boundaries);
+    query head g reads KV head g // (q_heads // num_kv_heads). cache_k / cache_v / k_scale / v_scale as
+    in qk_norm_rope_fill; page_table int32 [batch, max_num_blocks_per_seq]; seq_lens int32 [batch], the
+    new token included (its K and V are in the cache). Request b attends to the tokens below seq_lens[b]
+    that have a page (entry > 0), the last `window` of them where given, with scale (head_dim ** -0.5 if
+    None) on the scores. A request without tokens gets zeros and a log-sum-exp of -inf. Returns out
+    [batch, q_heads, head_dim], or (out, lse) with lse fp32 [batch, q_heads].
+
+    weights (fp32 [batch, num_kv_heads, tokens], covering the page table's tokens) accumulates what
+    evict_paged_kv chooses by: weights_out (default: weights itself) becomes weights plus each token's
+    softmax weight summed over the KV head's query heads, for the tokens below seq_lens. Equal calls
+    give equal bits. Asynchronous on the current stream; no backward pass."""
+    torch = _torch()
+    cache = _paged_cache(cache_k, cache_v, page_table, k_scale, v_scale)
+    dev = cache_k.device
+    _on(dev, q=q, seq_lens=seq_lens, out=out, weights=weights, weights_out=weights_out)
+    _rows("q", q, 3)
+    batch, q_heads, dim = q.shape
+    if batch != page_table.shape[0] or dim != cache_k.shape[3]:
+        raise RuntimeError("q must be [batch_size, q_heads, head_dim] of the page table's requests and the cache's head_dim")
+    _int32(1, seq_lens=seq_lens)
+    if seq_lens.shape[0] != batch:
+        raise RuntimeError(f"seq_lens size ({seq_lens.shape[0]}) must match batch_size ({batch})")
+    if window is not None and not 0 < window < 1 << 31:
+        raise RuntimeError("window must be 1 to 2^31 - 1 tokens")
+    if out is None:
+        out = torch.empty((batch, q_heads, dim), dtype=q.dtype, device=dev)
+    else:
+        _rows("out", out, 3)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise RuntimeError("out must have q's shape and dtype")
+    rows = _native.DecodeRows(q.data_ptr(), out.data_ptr(), _S2(*_strides(q, 2, 2)), _S2(*_strides(out, 2, 2)),
+                              seq_lens.data_ptr())
+    rows.q_heads, rows.dtype = q_heads, _dtype_code(q.dtype)
+    rows.window = window or 0
+    rows.scale = dim ** -0.5 if scale is None else scale
+    lse = None
+    if return_lse:
+        lse = torch.empty((batch, q_heads), dtype=torch.float32, device=dev)
+        rows.lse = lse.data_ptr()
+    if weights is not None:
+        weights_out = weights if weights_out is None else weights_out
+        cover = page_table.shape[1] * cache_k.shape[2]
+        _weight_sums("weights", weights, batch, cache_k.shape[1], cover)
+        _weight_sums("weights_out", weights_out, batch, cache_k.shape[1], cover)
+        rows.weights, rows.weights_out = weights.data_ptr(), weights_out.data_ptr()
+        rows.weights_strides = _S2(*_strides(weights, 2, 1))
+        rows.weights_out_strides = _S2(*_strides(weights_out, 2, 1))
+        rows.w_len = min(weights.shape[2], weights_out.shape[2])
+    elif weights_out is not None:
+        raise RuntimeError("weights_out needs weights")
+    lib = load()
+    need = C.c_uint64()
+    check(lib.kvs_decode_attention_workspace(C.byref(cache), C.byref(rows), dev.index, C.byref(need)))
+    workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    rows.workspace, rows.workspace_bytes = workspace.data_ptr(), need.value
+    check(lib.kvs_paged_decode_attention(C.byref(cache), C.byref(rows), _stream(dev)))
+    return (out, lse) if return_lse else out
+
+
+def evict_paged_kv(cache_k: Any, cache_v: Any, page_table: Any, seq_lens: Any, weights: Any, keep: int, *,
+                   first: int = 0, recent: int = 0, dst_page_table: Any = None, weights_out: Any = None,
+                   out_of_range: Any = None):
+    """Trim paged caches to the tokens that attention reads most. Returns (kept, new_lens).
+
+    Per request and KV head, of the tokens below seq_lens that have a page: the first `first` and the
+    last `recent` positions stay, and of the others those of the largest weight (equal weights: the
+    lowest position; NaN counts as the largest), `keep` in all. kept: int32 [batch, num_kv_heads, keep],
+    the kept positions in order, then -1; new_lens: int32 [batch], min(keep, tokens).
+
+    The kept rows move in order to slots 0, 1, ... of dst_page_table (int32 [batch, blocks], covering
+    keep slots), fresh pages that no table of the call reads, so pages shared between requests or held
+    by a store stay as they are. Without dst_page_table (or with page_table itself) they move within the
+    request's own pages, which then no other request may share. A slot without a valid page stores
+    nothing and is counted in out_of_range (int32, one element). weights: fp32 [batch, num_kv_heads,
+    tokens] as paged_decode_attention accumulates them, covering the page table's tokens; weights_out
+    (default: weights itself) receives the kept tokens' weights, then zeros up to seq_lens. Keys keep the
+    rotation of their old positions: rotate new tokens by the `positions` of qk_norm_rope_fill.
+    Asynchronous on the current stream."""
+    torch = _torch()
+    cache = _paged_cache(cache_k, cache_v, page_table, 1.0, 1.0)
+    dev = cache_k.device
+    weights_out = weights if weights_out is None else weights_out
+    _on(dev, seq_lens=seq_lens, weights=weights, dst_page_table=dst_page_table, weights_out=weights_out,
+        out_of_range=out_of_range)
+    _int32(1, seq_lens=seq_lens)
+    _int32(2, dst_page_table=dst_page_table)
+    batch, heads = page_table.shape[0], cache_k.shape[1]
+    if seq_lens.shape[0] != batch:
+        raise RuntimeError(f"seq_lens size ({seq_lens.shape[0]}) must match batch_size ({batch})")
+    if dst_page_table is not None and dst_page_table.shape[0] != batch:
+        raise RuntimeError(f"dst_page_table must have batch_size ({batch}) rows")
+    if keep <= 0 or keep >= 1 << 31 or first < 0 or recent < 0 or first + recent > keep:
+        raise RuntimeError(f"keep ({keep}) must be 1 to 2^31 - 1, first ({first}) and recent ({recent}) not negative and "
+                           "first + recent <= keep")
+    cover = page_table.shape[1] * cache_k.shape[2]
+    _weight_sums("weights", weights, batch, heads, cover)
+    _weight_sums("weights_out", weights_out, batch, heads, cover)
+    _check_counter(out_of_range)
+    kept = torch.empty((batch, heads, keep), dtype=torch.int32, device=dev)
+    new_lens = torch.empty((batch,), dtype=torch.int32, device=dev)
+    in_place = dst_page_table is None or dst_page_table.data_ptr() == page_table.data_ptr()
+    rows = _native.EvictRows(
+        seq_lens.data_ptr(), None if in_place else dst_page_table.data_ptr(), weights.data_ptr(),
+        weights_out.data_ptr(), _S2(*_strides(weights, 2, 1)), _S2(*_strides(weights_out, 2, 1)), kept.data_ptr(),
+        new_lens.data_ptr(), _ptr(out_of_range), 0 if in_place else dst_page_table.shape[1], weights.shape[2],
+        weights_out.shape[2], keep, first, recent)
+    check(load().kvs_evict_paged(C.byref(cache), C.byref(rows), _stream(dev)))
+    return kept, new_lens
