@@ -38,39 +38,71 @@ namespace kvs {
 
 namespace {
 
-constexpr int kWarps = 4;
+#ifndef TUNE_WARPS
+#define TUNE_WARPS 4
+#endif
+constexpr int kWarps = TUNE_WARPS;
 constexpr int kThreads = 32 * kWarps;
 constexpr uint32_t kTile = 16;       // tokens per warp tile
-constexpr uint32_t kUnitTiles = 16;  // tiles per unit of work: 256 tokens, 4 tiles per warp
+#ifndef TUNE_UNIT
+#define TUNE_UNIT 4
+#define TUNE_LEAST 4
+#define TUNE_WHOLE 512
+#endif
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 enum Kind { kKindBf16, kKindFp16, kKindE4m3 };
 
+// How a kernel streams: 16-token tiles per step, steps in the ring, bytes of a warp's ring and CTAs
+// per SM, by bytes per element, padded head_dim and column tiles of 8 heads.
+struct Shape {
+  int sub, stages, ring, ctas;
+};
+#ifndef TUNE_SUB
+#define TUNE_SUB (el == 2 && dp == 64 && nt == 1 ? 2 : 1)
+#define TUNE_BYTES (el == 1 && dp * nt <= 128 || el * dp * nt == 256 && dp == 64 ? 49152 : 98304)
+#define TUNE_CTAS (el == 1 && dp * nt <= 128 || el * dp * nt == 256 && dp == 64 ? 4 : 2)
+#endif
+__host__ __device__ constexpr Shape shape_of(int el, int dp, int nt) {
+  Shape s{};
+  s.sub = TUNE_SUB;
+  const int stage = 2 * 16 * s.sub * dp * el;
+  const int fit = TUNE_BYTES / (kWarps * stage);
+  s.stages = fit < 3 ? 3 : (fit > 8 ? 8 : fit);
+  s.ring = kWarps * s.stages * stage;
+  s.ctas = s.ring > 110 * 1024 ? 1 : TUNE_CTAS;
+  return s;
+}
+
 template <int kKind, int DP, int NT>
 struct Cfg {
   static constexpr int el = kKind == kKindE4m3 ? 1 : 2;
-  static constexpr int pitch = DP * el;                // bytes of a row in shared memory
-  static constexpr int chunks = pitch / 16;            // 16-byte pieces of a row
-  static constexpr int stage = 2 * (int)kTile * pitch; // K and V of one tile
-  static constexpr int fit = 98304 / (kWarps * stage);
-  static constexpr int stages = fit < 3 ? 3 : (fit > 8 ? 8 : fit);
-  static constexpr int ring = kWarps * stages * stage;
-  static constexpr int ctas = ring > 100 * 1024 ? 1 : 2;  // resident CTAs per SM
+  static constexpr Shape shape = shape_of(el, DP, NT);
+  static constexpr int pitch = DP * el;                 // bytes of a row in shared memory
+  static constexpr int chunks = pitch / 16;             // 16-byte pieces of a row
+  static constexpr int sub = shape.sub;
+  static constexpr uint32_t tokens = 16 * sub;
+  static constexpr int stage = 2 * (int)tokens * pitch; // K and V of one step
+  static constexpr int stages = shape.stages;
+  static constexpr int ring = shape.ring;
+  static constexpr int ctas = shape.ctas;
+  static constexpr int merge = NT * (DP / 16) * 512;    // one warp's accumulators
+  static constexpr int smem = ring + merge + 512;       // the ring starts on a row boundary
   static constexpr int heads = 8 * NT;
-  static constexpr int opitch = DP + 4;                // floats of a merged output row: conflict-free
-  static_assert(kWarps * heads * opitch * 4 <= ring, "the warps' outputs are merged in the ring");
 };
 
-// One head's partial over one CTA's tokens; a CTA leaves at most two (its first run continues an
-// earlier CTA's, its last run goes on in the next).
+// A (request, head tile) whose first units this CTA took and that goes on in `followers` more. A CTA
+// leaves at most two partials: slot 1 where its last run goes on, slot 0 where its first run continues
+// an earlier CTA's. A partial's accumulators lie in the order of the matrix fragments.
 struct Join {
   uint32_t b, hh, followers, pad;
 };
 
 struct Plan {  // workspace layout
   uint64_t joins, part_o, part_ml, lse2, logits, bytes;
-  uint32_t grid, head_tiles, tile_heads;
+  uint32_t grid, head_tiles, tile_heads, unit_tiles, least_units;
+  bool joins_needed;
 };
 
 __host__ __device__ inline uint32_t head_tiles_of(uint32_t group) { return (group + 15) / 16; }
@@ -83,12 +115,17 @@ Plan plan_of(const PagedCache &c, uint32_t q_heads, bool weights, int sms) {
   p.head_tiles = head_tiles_of(group);
   p.tile_heads = group <= 8 ? 8 : 16;
   const uint32_t dp = padded_dim(c.head_dim);
-  const uint32_t per_sm = dp == 256 && c.dtype != kE4m3 ? 1 : 2;
+  const uint32_t per_sm = shape_of(c.dtype == kE4m3 ? 1 : 2, dp, p.tile_heads / 8).ctas;
   const uint64_t cap = (uint64_t)c.max_blocks * c.block_size;
-  const uint64_t units = (cap + kTile * kUnitTiles - 1) / (kTile * kUnitTiles);
-  const uint64_t most = (uint64_t)c.batch * c.n_heads * p.head_tiles * units;
+  const uint32_t cap_tiles = (uint32_t)((cap + kTile - 1) / kTile);
+  const bool whole = cap <= TUNE_WHOLE;
+  p.unit_tiles = whole ? cap_tiles : TUNE_UNIT;
+  p.least_units = whole ? 1 : TUNE_LEAST;
+  const uint64_t units = (cap_tiles + p.unit_tiles - 1) / p.unit_tiles;
+  const uint64_t most = ((uint64_t)c.batch * c.n_heads * p.head_tiles * units + p.least_units - 1) / p.least_units;
   const uint64_t full = (uint64_t)sms * per_sm;
   p.grid = (uint32_t)(most < full ? most : full);
+  p.joins_needed = units > 1 && p.grid > 1;
   uint64_t off = 0;
   auto take = [&](uint64_t n) {
     const uint64_t o = off;
@@ -111,7 +148,8 @@ struct KernelParams {
   float2 *part_ml;
   float *lse2;    // base-2 log-sum-exp per row, kept for the weights
   float *logits;  // [batch][n_heads][cap][group] scores in base 2, or nullptr
-  uint32_t cap, head_tiles, group;
+  uint32_t cap, head_tiles, group, unit_tiles, least_units;
+  Divisor page;  // block_size
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -119,6 +157,9 @@ __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {
   // src-size 0 reads nothing and writes zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int n>
@@ -166,9 +207,9 @@ __device__ __forceinline__ uint32_t widen(uint32_t x) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"((uint16_t)x));
   return y;
 }
-__device__ __forceinline__ float load_elem(const uint8_t *row, uint32_t d, int32_t dtype) {
-  return dtype == kBf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(row)[d])
-                        : __half2float(reinterpret_cast<const __half *>(row)[d]);
+__device__ __forceinline__ float2 pair_of(uint32_t x, bool bf) {
+  if (bf) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2 *>(&x));
 }
 __device__ __forceinline__ void store_elem(uint8_t *row, uint32_t d, float x, int32_t dtype) {
   if (dtype == kBf16) reinterpret_cast<__nv_bfloat16 *>(row)[d] = __float2bfloat16_rn(x);
@@ -189,8 +230,39 @@ __device__ __forceinline__ Span span_of(const KernelParams &p, uint32_t b) {
   if (s.low > s.len) s.low = s.len;
   s.first = s.low / kTile;
   s.tiles = s.len > s.low ? (s.len + kTile - 1) / kTile - s.first : 0;
-  s.units = max(1u, (s.tiles + kUnitTiles - 1) / kUnitTiles);  // an empty row still gets its zeros written
+  s.units = max(1u, (s.tiles + p.unit_tiles - 1) / p.unit_tiles);  // an empty row still gets its zeros written
   return s;
+}
+
+__device__ __forceinline__ void store_lse(const KernelParams &p, uint64_t row, float m, float l) {
+  const float lse2 = l == 0.f ? -INFINITY : m + __log2f(l);
+  if (p.a.lse) p.a.lse[row] = lse2 * kLn2;
+  if (p.lse2) p.lse2[row] = lse2;
+}
+
+// Where a CTA is in its run of units: unit `unit` of head tile `hh` of request `b`, `left` units to go.
+struct Cursor {
+  uint32_t b, hh, unit;
+  uint64_t left;
+  Span span;
+  __device__ __forceinline__ uint32_t take() const { return (uint32_t)min((uint64_t)(span.units - unit), left); }
+  __device__ __forceinline__ uint32_t begin(const KernelParams &p) const { return span.first + unit * p.unit_tiles; }
+  __device__ __forceinline__ uint32_t end(const KernelParams &p) const { return span.first + min(span.tiles, (unit + take()) * p.unit_tiles); }
+  __device__ __forceinline__ void next(const KernelParams &p, uint32_t hh_n) {
+    left -= take();
+    unit = 0;
+    if (++hh == hh_n) {
+      hh = 0;
+      ++b;
+      if (left) span = span_of(p, b);
+    }
+  }
+};
+
+// Factor that brings sums relative to maximum m to maximum M (sums without a token are zero; a NaN
+// stays one).
+__device__ __forceinline__ float rebase(float m, float l, float M) {
+  return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2_fast(m - M);
 }
 
 template <int kKind, int DP, int NT>
@@ -199,11 +271,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
   constexpr bool kBf = kKind == kKindBf16;
   constexpr bool k8 = kKind == kKindE4m3;
   constexpr int kSteps = DP / 16;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t s_scan[kWarps + 2];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *const smem = smem_raw + (-smem_addr(smem_raw) & 511);
+  __shared__ uint64_t s_scan[kWarps + 1];
   __shared__ uint32_t s_where[2];
-  __shared__ uint32_t s_mask[kWarps][C::stages];
-  __shared__ float s_m[kWarps][C::heads], s_l[kWarps][C::heads], s_f[kWarps][C::heads], s_M[C::heads], s_L[C::heads];
+  __shared__ uint32_t s_mask[kWarps][C::stages][C::sub];
+  __shared__ float s_m[C::heads], s_l[C::heads];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedCache &c = p.a.c;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -222,13 +295,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
   total = 0;
   for (int w = 0; w < kWarps; ++w) total += s_scan[w];
   total *= hh_n;
-  const uint64_t quota = (total + gridDim.x - 1) / gridDim.x;
+  const uint64_t quota = max((uint64_t)p.least_units, (total + gridDim.x - 1) / gridDim.x);
   const uint64_t begin = quota * blockIdx.x;
-  if (begin >= total) {
-    if (tid == 0) p.joins[blockIdx.x].followers = 0;
-    return;
-  }
-  uint64_t left = min(quota, total - begin);
+  if (tid == 0) p.joins[blockIdx.x].followers = 0;
+  if (begin >= total) return;
   // request that holds unit `begin`: the requests' units times hh_n, scanned kThreads at a time
   uint64_t run = 0;
   for (uint32_t base = 0; base < c.batch; base += kThreads) {
@@ -257,132 +327,191 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
     __syncthreads();
     if (run * hh_n > begin) break;
   }
-  uint32_t b = s_where[0], hh = s_where[1];
-  uint32_t unit = (uint32_t)s_scan[kWarps];
-  Span span = span_of(p, b);
-  if (tid == 0) p.joins[blockIdx.x].followers = 0;
+  // The loads run ahead of the products, across the ends of runs: `ahead` is where the loads are.
+  Cursor at{s_where[0], s_where[1], (uint32_t)s_scan[kWarps], min(quota, total - begin), {}};
+  at.span = span_of(p, at.b);
+  Cursor ahead = at;
 
   const uint32_t ring = smem_addr(smem) + warp * C::stages * C::stage;
   const uint32_t row_chunks = (c.head_dim * C::el + 15) / 16;
-  const uint32_t used = k8 ? (c.head_dim + 31) / 32 * 32 : (c.head_dim + 15) / 16 * 16;  // elements the products run over
-  const uint32_t used_chunks = used * C::el / 16;
   const bool one_page = c.block_size % kTile == 0;  // a tile lies in one page
   const float scale2 = p.a.scale * c.k_scale * kLog2e;
-  // the pieces of a row this lane moves: piece lane % chunks of rows lane / chunks + i * rows_step
-  constexpr uint32_t rows_step = C::chunks >= 32 ? 1 : 32 / C::chunks;
+  // The pieces of a tile this lane moves: piece lane % chunks of the rows lane / chunks + i * rows_step.
+  // In shared memory piece j of row r sits at place j ^ swizzle(r) of the row, so that the eight rows
+  // of a matrix load fall on different banks; the swizzle of a sum of disjoint bits is the xor of
+  // theirs, which makes all but one term of each address a constant.
+  constexpr uint32_t rows_step = 32 / C::chunks;
+  static_assert(C::chunks <= 32, "a row is at most 512 bytes");
   const uint32_t my_chunk = lane % C::chunks, my_row = lane / C::chunks;
-  auto swizzle = [](uint32_t row) -> uint32_t { return C::pitch >= 128 ? (row & 7) : ((row >> 1) & 3); };
+  auto swizzle = [](uint32_t row) constexpr -> uint32_t { return C::pitch >= 128 ? (row & 7) : ((row >> 1) & 3); };
+  const uint32_t my_place = my_row * C::pitch + ((my_chunk ^ swizzle(my_row)) << 4);
 
-  while (left) {
-    const uint32_t take = (uint32_t)min((uint64_t)(span.units - unit), left);
-    const bool starts = unit == 0, ends = unit + take == span.units;
-    const uint32_t t_begin = span.first + unit * kUnitTiles;
-    const uint32_t t_end = span.first + min(span.tiles, (unit + take) * kUnitTiles);
-    const uint32_t h = hh / p.head_tiles, g0 = (hh % p.head_tiles) * C::heads;
-    const uint32_t heads = min((uint32_t)C::heads, p.group - g0);
-    const uint8_t *kh = c.k + (int64_t)h * c.k_head, *vh = c.v + (int64_t)h * c.v_head;
-    const int32_t *table = c.page_table + (uint64_t)b * c.max_blocks;
-
-    // page of this lane's token of a tile (of the tile, where it lies in one page); 0: masked
-    auto page_at = [&](uint32_t tile) -> int32_t {
-      if (tile >= t_end) return 0;
-      const uint32_t t = tile * kTile + (one_page ? 0 : (lane & 15));
-      const uint32_t vb = t / c.block_size;
-      if (vb >= c.max_blocks) return 0;
-      const int32_t pg = __ldg(table + vb);
-      return pg > 0 && (uint32_t)pg < c.num_blocks ? pg : 0;
-    };
-    auto issue = [&](uint32_t tile, uint32_t stage, int32_t page) {
-      if (tile < t_end) {
-        const uint32_t t0 = tile * kTile;
-        const uint32_t kdst = ring + stage * C::stage, vdst = kdst + kTile * C::pitch;
-        uint32_t mask = 0xFFFFu;
-        if (t0 + kTile > span.len) mask &= 0xFFFFu >> (t0 + kTile - span.len);
-        if (t0 < span.low) mask &= 0xFFFFu << (span.low - t0);
-        int64_t ko = 0, vo = 0;
-        if (one_page) {
-          if (page == 0) mask = 0;
-          const uint32_t r = t0 % c.block_size;
-          ko = (int64_t)page * c.k_page + (int64_t)r * c.k_row;
-          vo = (int64_t)page * c.v_page + (int64_t)r * c.v_row;
-        } else {
-          mask &= __ballot_sync(~0u, page != 0) & 0xFFFFu;
-          const uint32_t r = (t0 + (lane & 15)) % c.block_size;
-          ko = (int64_t)page * c.k_page + (int64_t)r * c.k_row;
-          vo = (int64_t)page * c.v_page + (int64_t)r * c.v_row;
-        }
-        if (lane == 0) s_mask[warp][stage] = mask;
+  // ---- loads
+  constexpr uint32_t stride = kWarps * C::sub;  // tiles between a warp's steps
+  uint32_t load_tile_at = ahead.begin(p) + warp * C::sub, load_end = ahead.end(p);
+  int32_t pages[C::sub];  // of the tiles of the next step to load; 0: masked
+  uint32_t slots[C::sub]; // this lane's token's (the tile's first token's) slot in its page
+  const uint8_t *kh, *vh; // this KV head's rows; this lane's piece of them where a tile lies in one page
+  auto find_head = [&]() {
+    const uint32_t h = ahead.hh / p.head_tiles;
+    kh = c.k + (int64_t)h * c.k_head + my_chunk * 16;
+    vh = c.v + (int64_t)h * c.v_head + my_chunk * 16;
+  };
+  auto find_pages = [&]() {
 #pragma unroll
-        for (int x = 0; x < C::chunks / 2; ++x) {
-          constexpr uint32_t per_row = C::chunks >= 32 ? C::chunks / 32 : 1;  // always 1 for rows up to 512 bytes
-          static_assert(per_row == 1, "a row is at most 512 bytes");
-          const uint32_t row = my_row + x * rows_step;
-          const bool there = (mask >> row) & 1 && my_chunk < row_chunks;
-          int64_t kro, vro;
-          if (one_page) {
-            kro = ko + (int64_t)row * c.k_row;
-            vro = vo + (int64_t)row * c.v_row;
-          } else {
-            kro = __shfl_sync(~0u, ko, row);
-            vro = __shfl_sync(~0u, vo, row);
-          }
-          if (!there) kro = vro = 0;  // the address of a row that is not read stays inside the cache
-          if (my_chunk < used_chunks) {
-            const uint32_t at = row * C::pitch + ((my_chunk ^ swizzle(row)) << 4);
-            const uint32_t src = there ? my_chunk * 16 : 0;
-            cp16(kdst + at, kh + kro + src, there);
-            cp16(vdst + at, vh + vro + src, there);
-          }
-        }
+    for (int u = 0; u < C::sub; ++u) {
+      pages[u] = 0;
+      slots[u] = 0;
+      const uint32_t tile = load_tile_at + u;
+      if (tile >= load_end) continue;
+      // page of this lane's token (of the whole tile, where it lies in one page)
+      const uint32_t t = tile * kTile + (one_page ? 0 : (lane & 15)), vb = p.page.quotient(t);
+      slots[u] = p.page.rest(t, vb);
+      if (vb >= c.max_blocks) continue;
+      const int32_t pg = __ldg(c.page_table + (uint64_t)ahead.b * c.max_blocks + vb);
+      pages[u] = pg > 0 && (uint32_t)pg < c.num_blocks ? pg : 0;
+    }
+  };
+  // to the next step of this warp, through runs that have none for it
+  auto settle = [&]() {
+    while (load_tile_at >= load_end && ahead.left) {
+      ahead.next(p, hh_n);
+      if (!ahead.left) break;
+      load_tile_at = ahead.begin(p) + warp * C::sub;
+      load_end = ahead.end(p);
+      find_head();
+    }
+    if (ahead.left) find_pages();
+  };
+  // one tile of K and V into shared memory, and which of its tokens count
+  auto load_tile = [&](uint32_t tile, uint32_t kdst, uint32_t vdst, int32_t page, uint32_t slot, uint32_t *note) {
+    const uint32_t t0 = tile * kTile;
+    uint32_t mask = tile < load_end ? 0xFFFFu : 0u;
+    if (t0 + kTile > ahead.span.len && mask) mask = 0xFFFFu >> min(16u, t0 + kTile - ahead.span.len);
+    if (t0 < ahead.span.low) mask &= 0xFFFFu << (ahead.span.low - t0);
+    if (one_page) mask = page ? mask : 0;
+    else mask &= __ballot_sync(~0u, page != 0);
+    if (lane == 0) *note = mask;
+    if (one_page && mask == 0xFFFFu) {
+      if (my_chunk >= row_chunks) return;
+      const uint8_t *ks = kh + (int64_t)page * c.k_page + (int64_t)(slot + my_row) * c.k_row;
+      const uint8_t *vs = vh + (int64_t)page * c.v_page + (int64_t)(slot + my_row) * c.v_row;
+      const int64_t kstep = rows_step * c.k_row, vstep = rows_step * c.v_row;
+#pragma unroll
+      for (uint32_t x = 0; x < kTile / rows_step; ++x) {
+        const uint32_t to = (my_place ^ (swizzle(x * rows_step) << 4)) + x * rows_step * C::pitch;
+        cp16(kdst + to, ks);
+        cp16(vdst + to, vs);
+        ks += kstep;
+        vs += vstep;
       }
-      cp_commit();
-    };
+      return;
+    }
+    const int64_t ko = (int64_t)page * c.k_page + (int64_t)slot * c.k_row;
+    const int64_t vo = (int64_t)page * c.v_page + (int64_t)slot * c.v_row;
+#pragma unroll
+    for (uint32_t x = 0; x < kTile / rows_step; ++x) {
+      const uint32_t row = my_row + x * rows_step;
+      int64_t kro = one_page ? ko + (int64_t)row * c.k_row : __shfl_sync(~0u, ko, row);
+      int64_t vro = one_page ? vo + (int64_t)row * c.v_row : __shfl_sync(~0u, vo, row);
+      const bool there = (mask >> row) & 1;
+      kro = there ? kro : -(int64_t)my_chunk * 16;  // the address of a piece that is not read stays inside the cache
+      vro = there ? vro : -(int64_t)my_chunk * 16;
+      if (my_chunk < row_chunks) {
+        const uint32_t to = (my_place ^ (swizzle(x * rows_step) << 4)) + x * rows_step * C::pitch;
+        cp16(kdst + to, kh + kro, there);
+        cp16(vdst + to, vh + vro, there);
+      }
+    }
+  };
+  // one step's loads; past the last step the group is empty, so that groups keep counting
+  auto issue = [&](uint32_t stage) {
+    if (ahead.left) {
+      const uint32_t kdst = ring + stage * C::stage, vdst = kdst + C::tokens * C::pitch;
+#pragma unroll
+      for (int u = 0; u < C::sub; ++u)
+        load_tile(load_tile_at + u, kdst + u * kTile * C::pitch, vdst + u * kTile * C::pitch, pages[u], slots[u], &s_mask[warp][stage][u]);
+      load_tile_at += stride;
+      settle();
+    }
+    cp_commit();
+  };
+  // Rows shorter than the padded head_dim: the products run over zeros behind them, which no load
+  // overwrites.
+  if (row_chunks < C::chunks)
+    for (uint32_t row = lane; row < C::stages * 2 * C::tokens; row += 32)
+      for (uint32_t j = row_chunks; j < C::chunks; ++j)
+        *reinterpret_cast<uint4 *>(smem + warp * C::stages * C::stage + row * C::pitch + ((j ^ swizzle(row)) << 4)) = make_uint4(0, 0, 0, 0);
+  find_head();
+  settle();
+#pragma unroll
+  for (int s = 0; s < C::stages - 1; ++s) issue(s);
+  uint32_t stage = 0;
+  const uint32_t k_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_row = (lane & 7) + (lane >> 4) * 8;
+  const uint32_t k_place = k_row * C::pitch + (((lane >> 4) ^ swizzle(k_row)) << 4);
+  const uint32_t v_place = v_row * C::pitch + ((((lane >> 3) & 1) ^ swizzle(v_row)) << 4);
 
-    // ---- queries: column fragments of Q^T, heads as columns
-    uint32_t bq[kSteps][NT][2];
-    float head_scale[NT][2];  // per column of the score tile (heads 2j, 2j + 1)
-    {
-      const uint32_t j = lane & 3, n = lane >> 2;
+  uint32_t bq[kSteps][NT][2];
+  // Queries of a run, as they are in memory. The product's index 2j + {0, 1} of a step is element
+  // 2j + {0, 1} (and 2j + 8 + {0, 1} eight further on); for an e4m3 cache 4j + {0, 1} (4j + 2 + {0, 1}),
+  // the order in which four bytes of a key row come out of a matrix load.
+  auto load_queries = [&](const Cursor &of) {
+    const uint32_t first_head = of.hh / p.head_tiles * p.group, g_first = of.hh % p.head_tiles * C::heads;
+    const uint32_t j = lane & 3;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const uint32_t g = nt * 8 + n;
-        const uint8_t *qr = p.a.q + (int64_t)b * p.a.q_req + (int64_t)(h * p.group + g0 + g) * p.a.q_head;
-        const bool live = g < heads;
-        if (!k8) {
-          head_scale[nt][0] = head_scale[nt][1] = scale2;
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint32_t g = g_first + nt * 8 + (lane >> 2);
+      const uint32_t *qr = reinterpret_cast<const uint32_t *>(p.a.q + (int64_t)of.b * p.a.q_req + (int64_t)(first_head + g) * p.a.q_head);
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s)
+      for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t d = 16 * s + 8 * half + 2 * j;
-              bq[s][nt][half] = live && d < c.head_dim ? __ldg(reinterpret_cast<const uint32_t *>(qr) + d / 2) : 0u;
-            }
-        } else {
-          // scaled by a power of two so that the head's largest element is in [1, 2): elements
-          // below 2^-14 of it lose at most 2^-25 of it
-          float big = 0.f;
-          for (uint32_t d = j; d < c.head_dim; d += 4)
-            if (live) big = fmaxf(big, fabsf(load_elem(qr, d, p.a.dtype)));
-          big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
-          big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
-          // both the factor 2^-e and 2^e have to be normal numbers
-          int e = big > 0.f && big < __int_as_float(0x7f800000) ? (int)(__float_as_uint(big) >> 23) - 127 : 0;
-          e = max(-126, min(126, e));
-          const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-          const float up = __uint_as_float((uint32_t)(127 + e) << 23) * scale2;
-          // k index 2j + {0, 1} of a step is element 4j + {0, 1}, 2j + 8 + {0, 1} is 4j + 2 + {0, 1}: the
-          // order in which four bytes of a key row come out of the matrix load
-#pragma unroll
-          for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t d = 16 * s + 4 * j + 2 * half;
-              const bool in = live && d < c.head_dim;
-              bq[s][nt][half] = in ? pack2<false>(load_elem(qr, d, p.a.dtype) * down, load_elem(qr, d + 1, p.a.dtype) * down) : 0u;
-            }
-          head_scale[nt][0] = __shfl_sync(~0u, up, 8 * j);
-          head_scale[nt][1] = __shfl_sync(~0u, up, 8 * j + 4);
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t d = k8 ? 16 * s + 4 * j + 2 * half : 16 * s + 8 * half + 2 * j;
+          bq[s][nt][half] = g < p.group && d < c.head_dim ? __ldg(qr + d / 2) : 0u;
         }
+    }
+  };
+  load_queries(at);
+
+  while (at.left) {
+    const uint32_t b = at.b, h = at.hh / p.head_tiles, g0 = (at.hh % p.head_tiles) * C::heads;
+    const uint32_t heads = min((uint32_t)C::heads, p.group - g0);
+    const uint32_t t_begin = at.begin(p), t_end = at.end(p);
+
+    // ---- queries (loaded before the last run's join): column fragments of Q^T, heads as columns
+    float head_scale[NT][2];  // per column of the score tile (heads 2j, 2j + 1)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (!k8) {
+        head_scale[nt][0] = head_scale[nt][1] = scale2;
+      } else {
+        // scaled by a power of two so that the head's largest element is in [1, 2), which fits fp16:
+        // elements below 2^-14 of it lose at most 2^-25 of it
+        const bool bf = p.a.dtype == kBf16;
+        float big = 0.f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float2 x = pair_of(bq[s][nt][half], bf);
+            big = fmaxf(big, fmaxf(fabsf(x.x), fabsf(x.y)));
+          }
+        big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
+        // both the factor 2^-e and 2^e have to be normal numbers
+        int e = big > 0.f && big < __int_as_float(0x7f800000) ? (int)(__float_as_uint(big) >> 23) - 127 : 0;
+        e = max(-126, min(126, e));
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23) * scale2;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float2 x = pair_of(bq[s][nt][half], bf);
+            bq[s][nt][half] = pack2<false>(x.x * down, x.y * down);
+          }
+        head_scale[nt][0] = __shfl_sync(~0u, up, 8 * (lane & 3));
+        head_scale[nt][1] = __shfl_sync(~0u, up, 8 * (lane & 3) + 4);
       }
     }
 
@@ -398,67 +527,79 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
         for (int i = 0; i < 4; ++i) acc[nt][s][i] = 0.f;
     }
 
-    uint32_t tile = t_begin + warp;
-#pragma unroll
-    for (int s = 0; s < C::stages - 1; ++s) issue(tile + s * kWarps, s, page_at(tile + s * kWarps));
-    int32_t next_page = page_at(tile + (C::stages - 1) * kWarps);
-    uint32_t stage = 0;
-    for (; tile < t_end; tile += kWarps) {
+    for (uint32_t tile = t_begin + warp * C::sub; tile < t_end; tile += stride) {
       cp_wait<C::stages - 2>();
       __syncwarp();
-      {
-        const uint32_t fresh = stage == 0 ? C::stages - 1 : stage - 1;
-        const uint32_t ahead = tile + (C::stages - 1) * kWarps;
-        issue(ahead, fresh, next_page);
-        next_page = page_at(ahead + kWarps);
-      }
-      const uint32_t kt = ring + stage * C::stage, vt = kt + kTile * C::pitch;
-      const uint32_t mask = s_mask[warp][stage];
+      issue(stage == 0 ? C::stages - 1 : stage - 1);
+      const uint32_t kt = ring + stage * C::stage + k_place, vt = ring + stage * C::stage + C::tokens * C::pitch + v_place;
 
-      // ---- S^T = K Q^T
-      float sc[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+      // ---- S^T = K Q^T (two chains of products per tile)
+      float sc[C::sub][NT][4];
       {
-        const uint32_t row = (lane & 7) + ((lane >> 3) & 1) * 8, ch = lane >> 4;
-        const uint32_t at = kt + row * C::pitch, sw = swizzle(row);
-        if (!k8) {
+        float sd[C::sub][NT][4];
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            if (16 * s >= used) break;
-            uint32_t a[4];
-            ldsm4(a, at + (((2 * s + ch) ^ sw) << 4));
+        for (int u = 0; u < C::sub; ++u)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma<kBf>(sc[nt], a[0], a[1], a[2], a[3], bq[s][nt][0], bq[s][nt][1]);
-          }
-        } else {
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int s = 0; s < kSteps; s += 2) {
-            if (16 * s >= used) break;
-            uint32_t a[4];
-            ldsm4(a, at + (((s + ch) ^ sw) << 4));
+            for (int i = 0; i < 4; ++i) sc[u][nt][i] = sd[u][nt][i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t x0 = widen(a[2 * i]), x1 = widen(a[2 * i + 1]), x2 = widen(a[2 * i] >> 16), x3 = widen(a[2 * i + 1] >> 16);
+        for (int s = 0; s < kSteps; s += 2) {
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt], x0, x1, x2, x3, bq[s + i][nt][0], bq[s + i][nt][1]);
+          for (int u = 0; u < C::sub; ++u) {
+            const uint32_t at = kt + u * kTile * C::pitch;
+            if (!k8) {
+              uint32_t a[4];
+              ldsm4(a, at ^ (s << 5));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma<kBf>(sc[u][nt], a[0], a[1], a[2], a[3], bq[s][nt][0], bq[s][nt][1]);
+              ldsm4(a, at ^ ((s + 1) << 5));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma<kBf>(sd[u][nt], a[0], a[1], a[2], a[3], bq[s + 1][nt][0], bq[s + 1][nt][1]);
+            } else {
+              uint32_t a[4];
+              ldsm4(a, at ^ (s << 4));
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t x0 = widen(a[2 * i]), x1 = widen(a[2 * i + 1]), x2 = widen(a[2 * i] >> 16), x3 = widen(a[2 * i + 1] >> 16);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma<false>(i ? sd[u][nt] : sc[u][nt], x0, x1, x2, x3, bq[s + i][nt][0], bq[s + i][nt][1]);
+              }
             }
           }
         }
+#pragma unroll
+        for (int u = 0; u < C::sub; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[u][nt][i] = (sc[u][nt][i] + sd[u][nt][i]) * head_scale[nt][i & 1];
       }
 
-      // ---- running maximum and sum; tokens lane / 4 and lane / 4 + 8, heads 2j and 2j + 1
-      const bool in0 = (mask >> (lane >> 2)) & 1, in1 = (mask >> ((lane >> 2) + 8)) & 1;
-      uint32_t pb[NT][2];
+      // ---- running maximum and sum; tokens lane / 4 and lane / 4 + 8 of each tile, heads 2j and 2j + 1
+#pragma unroll
+      for (int u = 0; u < C::sub; ++u) {
+        const uint32_t mask = s_mask[warp][stage][u];
+        if (mask != 0xFFFFu) {
+          const bool in0 = (mask >> (lane >> 2)) & 1, in1 = (mask >> ((lane >> 2) + 8)) & 1;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (!in0) sc[u][nt][i] = -INFINITY;
+              if (!in1) sc[u][nt][2 + i] = -INFINITY;
+            }
+        }
+      }
       bool grew = false;
       float mn[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          sc[nt][i] = in0 ? sc[nt][i] * head_scale[nt][i] : -INFINITY;
-          sc[nt][2 + i] = in1 ? sc[nt][2 + i] * head_scale[nt][i] : -INFINITY;
-          float x = fmaxf(sc[nt][i], sc[nt][2 + i]);
+          float x = fmaxf(sc[0][nt][i], sc[0][nt][2 + i]);
+#pragma unroll
+          for (int u = 1; u < C::sub; ++u) x = fmaxf(x, fmaxf(sc[u][nt][i], sc[u][nt][2 + i]));
           x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
           x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
           x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
@@ -466,16 +607,25 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
           grew |= mn[nt][i] > m[nt][i];
         }
       if (p.logits) {
-        float *lg = p.logits + (((uint64_t)b * c.n_heads + h) * p.cap + (uint64_t)tile * kTile + (lane >> 2)) * p.group + g0;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int u = 0; u < C::sub; ++u) {
+          const uint32_t t = (tile + u) * kTile + (lane >> 2);
+          float *lg = p.logits + (((uint64_t)b * c.n_heads + h) * p.cap + t) * p.group + g0;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t g = nt * 8 + 2 * (lane & 3) + i;
-            const uint32_t t = tile * kTile + (lane >> 2);
-            if (g < heads && t < span.len) lg[g] = sc[nt][i];
-            if (g < heads && t + 8 < span.len) lg[8ull * p.group + g] = sc[nt][2 + i];
-          }
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t g = nt * 8 + 2 * (lane & 3);
+              if (t + 8 * i >= at.span.len || g >= heads) continue;
+              float *to = lg + 8ull * i * p.group + g;
+              if (p.group % 2 == 0) {
+                *reinterpret_cast<float2 *>(to) = make_float2(sc[u][nt][2 * i], sc[u][nt][2 * i + 1]);
+              } else {
+                to[0] = sc[u][nt][2 * i];
+                if (g + 1 < heads) to[1] = sc[u][nt][2 * i + 1];
+              }
+            }
+        }
       }
       if (__any_sync(~0u, grew)) {
 #pragma unroll
@@ -492,54 +642,52 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
             }
           }
       }
+      uint32_t pb[C::sub][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float e[4];
+        const float base0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], base1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float base = m[nt][i] == -INFINITY ? 0.f : m[nt][i];
-          e[i] = exp2_fast(sc[nt][i] - base);
-          e[2 + i] = exp2_fast(sc[nt][2 + i] - base);
-          l[nt][i] += e[i] + e[2 + i];
+        for (int u = 0; u < C::sub; ++u) {
+          const float e0 = exp2_fast(sc[u][nt][0] - base0), e1 = exp2_fast(sc[u][nt][1] - base1);
+          const float e2 = exp2_fast(sc[u][nt][2] - base0), e3 = exp2_fast(sc[u][nt][3] - base1);
+          l[nt][0] += e0 + e2;
+          l[nt][1] += e1 + e3;
+          pb[u][nt][0] = transpose8(pack2<kBf>(e0, e1));
+          pb[u][nt][1] = transpose8(pack2<kBf>(e2, e3));
         }
-        pb[nt][0] = transpose8(pack2<kBf>(e[0], e[1]));
-        pb[nt][1] = transpose8(pack2<kBf>(e[2], e[3]));
       }
 
       // ---- O^T += V^T P^T
-      {
-        const uint32_t row = (lane & 7) + (lane >> 4) * 8, ch = (lane >> 3) & 1;
-        const uint32_t at = vt + row * C::pitch, sw = swizzle(row);
+#pragma unroll
+      for (int u = 0; u < C::sub; ++u) {
+        const uint32_t at = vt + u * kTile * C::pitch;
         if (!k8) {
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
-            if (16 * s >= used) break;
             uint32_t a[4];
-            ldsm4t(a, at + (((2 * s + ch) ^ sw) << 4));
+            ldsm4t(a, at ^ (s << 5));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma<kBf>(acc[nt][s], a[0], a[1], a[2], a[3], pb[nt][0], pb[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma<kBf>(acc[nt][s], a[0], a[1], a[2], a[3], pb[u][nt][0], pb[u][nt][1]);
           }
         } else {
           // a transposed load of byte pairs gives (t0 d0, t0 d1, t1 d0, t1 d1): even elements become
           // rows 0-7 of the 16-element tile, odd ones rows 8-15
 #pragma unroll
           for (int s = 0; s < kSteps; s += 2) {
-            if (16 * s >= used) break;
             uint32_t a[4];
-            ldsm4t(a, at + (((s + ch) ^ sw) << 4));
+            ldsm4t(a, at ^ (s << 4));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t lo = __byte_perm(a[i], 0, 0x3120), hi = __byte_perm(a[2 + i], 0, 0x3120);
               const uint32_t x0 = widen(lo), x1 = widen(lo >> 16), x2 = widen(hi), x3 = widen(hi >> 16);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma<false>(acc[nt][s + i], x0, x1, x2, x3, pb[nt][0], pb[nt][1]);
+              for (int nt = 0; nt < NT; ++nt) mma<false>(acc[nt][s + i], x0, x1, x2, x3, pb[u][nt][0], pb[u][nt][1]);
             }
           }
         }
       }
       stage = stage + 1 == C::stages ? 0 : stage + 1;
     }
-    cp_wait<0>();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -549,136 +697,186 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
         l[nt][i] += __shfl_xor_sync(~0u, l[nt][i], 16);
       }
 
-    // ---- join the warps
-    __syncthreads();  // every warp has read its last tile: the ring becomes the outputs' buffer
-    float *so = reinterpret_cast<float *>(smem);
-    {
-      const uint32_t j = lane & 3, r = lane >> 2;
+    Cursor following = at;
+    following.next(p, hh_n);
+    if (following.left) load_queries(following);
+
+    // ---- warp 0 takes in the other warps' sums, one after the other (those that had a step)
+    float4 *const buf = reinterpret_cast<float4 *>(smem + C::ring);
+    for (uint32_t w = 1; w < kWarps; ++w) {
+      if (t_begin + w * C::sub >= t_end) break;
+      if (warp == w) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t g = nt * 8 + 2 * j + i;
-          float *row = so + (warp * C::heads + g) * C::opitch;
+          for (int s = 0; s < kSteps; ++s)
+            buf[(nt * kSteps + s) * 32 + lane] = make_float4(acc[nt][s][0], acc[nt][s][1], acc[nt][s][2], acc[nt][s][3]);
+          if (lane < 4) {
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            row[16 * s + (k8 ? 2 * r : r)] = acc[nt][s][i];
-            row[16 * s + (k8 ? 2 * r + 1 : r + 8)] = acc[nt][s][2 + i];
-          }
-          if (r == 0) {
-            s_m[warp][g] = m[nt][i];
-            s_l[warp][g] = l[nt][i];
+            for (int i = 0; i < 2; ++i) {
+              s_m[nt * 8 + 2 * lane + i] = m[nt][i];
+              s_l[nt * 8 + 2 * lane + i] = l[nt][i];
+            }
           }
         }
       }
-    }
-    __syncthreads();
-    if (tid < C::heads) {
-      float M = -INFINITY, L = 0.f;
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][tid]);
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = s_m[w][tid] == -INFINITY ? (s_l[w][tid] == 0.f ? 0.f : 1.f) : exp2_fast(s_m[w][tid] - M);
-        s_f[w][tid] = f;
-        L += f * s_l[w][tid];
-      }
-      s_M[tid] = M;
-      s_L[tid] = L;
-    }
-    __syncthreads();
-    const bool whole = starts && ends;
-    const uint32_t slot = 2 * blockIdx.x + (starts ? 1 : 0);
-    for (uint32_t e = tid; e < heads * DP; e += kThreads) {
-      const uint32_t g = e / DP, d = e % DP;
-      if (d >= c.head_dim) continue;
-      float x = 0.f;
+      __syncthreads();
+      if (warp == 0) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) x += s_f[w][g] * so[(w * C::heads + g) * C::opitch + d];
-      if (whole) {
-        const float L = s_L[g];
-        store_elem(p.a.out + (int64_t)b * p.a.o_req + (int64_t)(h * p.group + g0 + g) * p.a.o_head, d, L == 0.f ? 0.f : x / L * c.v_scale, p.a.dtype);
+        for (int nt = 0; nt < NT; ++nt) {
+          float f0[2], f1[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float mw = s_m[nt * 8 + 2 * (lane & 3) + i], lw = s_l[nt * 8 + 2 * (lane & 3) + i];
+            const float M = fmaxf(m[nt][i], mw);
+            f0[i] = rebase(m[nt][i], l[nt][i], M);
+            f1[i] = rebase(mw, lw, M);
+            m[nt][i] = M;
+            l[nt][i] = l[nt][i] * f0[i] + lw * f1[i];
+          }
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            const float4 x = buf[(nt * kSteps + s) * 32 + lane];
+            acc[nt][s][0] = acc[nt][s][0] * f0[0] + x.x * f1[0];
+            acc[nt][s][1] = acc[nt][s][1] * f0[1] + x.y * f1[1];
+            acc[nt][s][2] = acc[nt][s][2] * f0[0] + x.z * f1[0];
+            acc[nt][s][3] = acc[nt][s][3] * f0[1] + x.w * f1[1];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (warp == 0) {
+      const bool starts = at.unit == 0, ends = at.unit + at.take() == at.span.units;
+      if (starts && ends) {
+        const uint32_t r = lane >> 2;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t g = nt * 8 + 2 * (lane & 3) + i;
+            if (g >= heads) continue;
+            const float f = l[nt][i] == 0.f ? 0.f : c.v_scale / l[nt][i];
+            uint8_t *o = p.a.out + (int64_t)b * p.a.o_req + (int64_t)(h * p.group + g0 + g) * p.a.o_head;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+              const uint32_t d0 = 16 * s + (k8 ? 2 * r : r), d1 = 16 * s + (k8 ? 2 * r + 1 : r + 8);
+              if (d0 < c.head_dim) store_elem(o, d0, acc[nt][s][i] * f, p.a.dtype);
+              if (d1 < c.head_dim) store_elem(o, d1, acc[nt][s][2 + i] * f, p.a.dtype);
+            }
+            if (r == 0) store_lse(p, (uint64_t)b * p.a.q_heads + h * p.group + g0 + g, m[nt][i], l[nt][i]);
+          }
       } else {
-        p.part_o[((uint64_t)slot * C::heads + g) * DP + d] = x;
+        const uint64_t slot = 2ull * blockIdx.x + (starts ? 1 : 0);
+        float4 *po = reinterpret_cast<float4 *>(p.part_o) + slot * NT * kSteps * 32;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s)
+            po[(nt * kSteps + s) * 32 + lane] = make_float4(acc[nt][s][0], acc[nt][s][1], acc[nt][s][2], acc[nt][s][3]);
+          if (lane < 4) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) p.part_ml[slot * C::heads + nt * 8 + 2 * lane + i] = make_float2(m[nt][i], l[nt][i]);
+          }
+        }
+        // units of this (request, head tile) after the ones taken here, over runs of `quota`
+        if (lane == 0 && starts)
+          p.joins[blockIdx.x] = Join{b, at.hh, (uint32_t)((at.span.units - at.take() + quota - 1) / quota), 0};
       }
     }
-    if (tid < heads) {
-      if (whole) {
-        const float lse2 = s_L[tid] == 0.f ? -INFINITY : s_M[tid] + __log2f(s_L[tid]);
-        const uint64_t at = (uint64_t)b * p.a.q_heads + h * p.group + g0 + tid;
-        if (p.a.lse) p.a.lse[at] = lse2 * kLn2;
-        if (p.lse2) p.lse2[at] = lse2;
-      } else {
-        p.part_ml[(uint64_t)slot * C::heads + tid] = make_float2(s_M[tid], s_L[tid]);
-      }
-    }
-    if (tid == 0 && starts && !ends) {
-      // units of this (request, head tile) after the ones taken here, over runs of `quota`
-      const uint64_t rest = span.units - take;
-      p.joins[blockIdx.x] = Join{b, hh, (uint32_t)((rest + quota - 1) / quota), 0};
-    }
-    left -= take;
-    unit = 0;
-    if (++hh == hh_n && left) {
-      hh = 0;
-      ++b;
-      span = span_of(p, b);
-    }
-    __syncthreads();  // the buffer is a ring again
+    at = following;
   }
 }
 
 // Joins the partials of the (request, head tile) whose first units CTA blockIdx.x took: slot 1 of
-// that CTA, then slot 0 of the CTAs after it. One block per head.
-template <int DP>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ KernelParams p, uint32_t tile_heads) {
-  extern __shared__ float s_fac[];
-  __shared__ float s_red[8];
-  __shared__ float s_out[256];
+// that CTA, then slot 0 of the CTAs after it, in that order. One block per 16 elements of 8 heads (one
+// fragment), its eight warps taking every eighth partial.
+template <int DP, int NT, bool k8>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ KernelParams p) {
+  constexpr int kSteps = DP / 16;
+  constexpr uint32_t tile_heads = 8 * NT;
+  __shared__ float4 s_sum[8][32];
+  __shared__ float s_red[8][8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Join j = p.joins[blockIdx.x];
   if (j.followers == 0) return;
-  const uint32_t g = blockIdx.y, g0 = (j.hh % p.head_tiles) * tile_heads, h = j.hh / p.head_tiles;
-  if (g0 + g >= p.group) return;
-  const uint32_t n = j.followers + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t nt = blockIdx.y / kSteps, s = blockIdx.y % kSteps;
+  const uint32_t g0 = (j.hh % p.head_tiles) * tile_heads + nt * 8, h = j.hh / p.head_tiles;
+  if (g0 >= p.group || 16 * s >= p.a.c.head_dim) return;
+  const uint32_t n = j.followers + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto slot = [&](uint32_t i) -> uint64_t { return i == 0 ? 2ull * blockIdx.x + 1 : 2ull * (blockIdx.x + i); };
-  float M = -INFINITY;
-  for (uint32_t i = tid; i < n; i += 256) M = fmaxf(M, p.part_ml[slot(i) * tile_heads + g].x);
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
-  if (lane == 0) s_red[warp] = M;
-  __syncthreads();
-  for (int w = 0; w < 8; ++w) M = fmaxf(M, s_red[w]);
-  __syncthreads();
-  float L = 0.f;
-  for (uint32_t i = tid; i < n; i += 256) {
-    const float2 ml = p.part_ml[slot(i) * tile_heads + g];
-    const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - M);
-    s_fac[i] = f;
-    L += f * ml.y;
-  }
-  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
-  if (lane == 0) s_red[warp] = L;
-  __syncthreads();
-  L = 0.f;
-  for (int w = 0; w < 8; ++w) L += s_red[w];
-  // 256 / DP groups of threads take every (256 / DP)-th partial of an element
-  constexpr uint32_t parts = 256 / DP;
-  const uint32_t d = tid % DP, part = tid / DP;
-  float x = 0.f;
-  if (d < p.a.c.head_dim) {
-#pragma unroll 4
-    for (uint32_t i = part; i < n; i += parts) x += s_fac[i] * p.part_o[(slot(i) * tile_heads + g) * DP + d];
-  }
-  s_out[tid] = x;
-  __syncthreads();
-  const uint64_t head = h * p.group + g0 + g;
-  if (part == 0 && d < p.a.c.head_dim) {
+  // the first partials of each warp are on their way while the maxima are found
+  auto sums_of = [&](uint32_t i) {
+    return reinterpret_cast<const float4 *>(p.part_o)[(slot(i) * NT * kSteps + nt * kSteps + s) * 32 + lane];
+  };
+  auto stats_of = [&](uint32_t i) { return *reinterpret_cast<const float4 *>(p.part_ml + slot(i) * tile_heads + nt * 8 + 2 * (lane & 3)); };
+  constexpr int kEarly = 5;
+  float4 y[kEarly], ml[kEarly];
 #pragma unroll
-    for (uint32_t i = 1; i < parts; ++i) x += s_out[i * DP + d];
-    store_elem(p.a.out + (int64_t)j.b * p.a.o_req + (int64_t)head * p.a.o_head, d, L == 0.f ? 0.f : x / L * p.a.c.v_scale, p.a.dtype);
+  for (int e = 0; e < kEarly; ++e)
+    if (warp + 8 * e < n) {
+      y[e] = sums_of(warp + 8 * e);
+      ml[e] = stats_of(warp + 8 * e);
+    }
+  // maximum of each of the eight heads: lane % 8 is the head
+  float M = -INFINITY;
+  for (uint32_t i = warp * 4 + lane / 8; i < n; i += 32) M = fmaxf(M, p.part_ml[slot(i) * tile_heads + nt * 8 + lane % 8].x);
+  M = fmaxf(M, __shfl_xor_sync(~0u, M, 8));
+  M = fmaxf(M, __shfl_xor_sync(~0u, M, 16));
+  if (lane < 8) s_red[warp][lane] = M;
+  __syncthreads();
+  float top[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    top[i] = -INFINITY;
+    for (int w = 0; w < 8; ++w) top[i] = fmaxf(top[i], s_red[w][2 * (lane & 3) + i]);
   }
-  if (tid == 0) {
-    const float lse2 = L == 0.f ? -INFINITY : M + __log2f(L);
-    if (p.a.lse) p.a.lse[(uint64_t)j.b * p.a.q_heads + head] = lse2 * kLn2;
-    if (p.lse2) p.lse2[(uint64_t)j.b * p.a.q_heads + head] = lse2;
+  __syncthreads();
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  float L[2] = {0.f, 0.f};
+  auto add = [&](const float4 &o, const float4 &st) {
+    const float f0 = rebase(st.x, st.y, top[0]), f1 = rebase(st.z, st.w, top[1]);
+    x.x += f0 * o.x;
+    x.y += f1 * o.y;
+    x.z += f0 * o.z;
+    x.w += f1 * o.w;
+    L[0] += f0 * st.y;
+    L[1] += f1 * st.w;
+  };
+#pragma unroll
+  for (int e = 0; e < kEarly; ++e)
+    if (warp + 8 * e < n) add(y[e], ml[e]);
+#pragma unroll 4
+  for (uint32_t i = warp + 8 * kEarly; i < n; i += 8) add(sums_of(i), stats_of(i));
+  s_sum[warp][lane] = x;
+  if (lane < 4) {
+    s_red[warp][2 * lane] = L[0];
+    s_red[warp][2 * lane + 1] = L[1];
+  }
+  __syncthreads();
+  if (warp) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) {
+    const float4 y = s_sum[w][lane];
+    x.x += y.x;
+    x.y += y.y;
+    x.z += y.z;
+    x.w += y.w;
+    L[0] += s_red[w][2 * (lane & 3)];
+    L[1] += s_red[w][2 * (lane & 3) + 1];
+  }
+  const uint32_t r = lane >> 2;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t g = g0 + 2 * (lane & 3) + i;
+    if (g >= p.group) continue;
+    const uint64_t head = h * p.group + g;
+    const float f = L[i] == 0.f ? 0.f : p.a.c.v_scale / L[i];
+    uint8_t *o = p.a.out + (int64_t)j.b * p.a.o_req + (int64_t)head * p.a.o_head;
+    const uint32_t d0 = 16 * s + (k8 ? 2 * r : r), d1 = 16 * s + (k8 ? 2 * r + 1 : r + 8);
+    if (d0 < p.a.c.head_dim) store_elem(o, d0, (i ? x.y : x.x) * f, p.a.dtype);
+    if (d1 < p.a.c.head_dim) store_elem(o, d1, (i ? x.w : x.z) * f, p.a.dtype);
+    if (s == 0 && r == 0) store_lse(p, (uint64_t)j.b * p.a.q_heads + head, top[i], L[i]);
   }
 }
 
@@ -696,7 +894,16 @@ __global__ void __launch_bounds__(256) add_weights_kernel(const __grid_constant_
   float x = 0.f;
   if (t >= span.low) {
     const float *lg = p.logits + (((uint64_t)b * p.a.c.n_heads + h) * p.cap + t) * p.group;
-    for (uint32_t g = 0; g < p.group; ++g) x += s_lse[g] == -INFINITY ? 0.f : exp2_fast(lg[g] - s_lse[g]);
+    auto weight = [&](float score, uint32_t g) { return s_lse[g] == -INFINITY ? 0.f : exp2_fast(score - s_lse[g]); };
+    if (p.group % 4 == 0) {
+#pragma unroll 2
+      for (uint32_t g = 0; g < p.group; g += 4) {
+        const float4 y = *reinterpret_cast<const float4 *>(lg + g);
+        x += (weight(y.x, g) + weight(y.y, g + 1)) + (weight(y.z, g + 2) + weight(y.w, g + 3));
+      }
+    } else {
+      for (uint32_t g = 0; g < p.group; ++g) x += weight(lg[g], g);
+    }
   }
   p.a.weights_out[(int64_t)b * p.a.wo_req + (int64_t)h * p.a.wo_head + t] =
       p.a.weights[(int64_t)b * p.a.w_req + (int64_t)h * p.a.w_head + t] + x;
@@ -729,18 +936,16 @@ cudaError_t run(const KernelParams &kp, const Plan &plan, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const uint64_t bit = 1ull << (dev & 63);
   if (dev >= 64 || !(ready.load(std::memory_order_acquire) & bit)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::ring);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
     if (e != cudaSuccess) return e;
     if (dev < 64) ready.fetch_or(bit, std::memory_order_release);
   }
-  kernel<<<plan.grid, kThreads, C::ring, stream>>>(kp);
+  kernel<<<plan.grid, kThreads, C::smem, stream>>>(kp);
   count_launch();
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // a request of one unit is never split
-  if (kp.cap > kTile * kUnitTiles && plan.grid > 1) {
-    const uint32_t heads = kp.group < (uint32_t)C::heads ? kp.group : (uint32_t)C::heads;
-    e = launch_after(join_kernel<DP>, dim3(plan.grid, heads), dim3(256), 4ull * (plan.grid + 1), stream, kp, (uint32_t)C::heads);
+  if (plan.joins_needed) {
+    e = launch_after(join_kernel<DP, NT, kKind == kKindE4m3>, dim3(plan.grid, NT * (DP / 16)), dim3(256), 0, stream, kp);
     if (e != cudaSuccess) return e;
   }
   if (kp.logits) {
@@ -779,6 +984,9 @@ cudaError_t launch_decode_attention(const DecodeAttentionParams &a, int sms, cud
   kp.part_ml = reinterpret_cast<float2 *>(a.workspace + plan.part_ml);
   kp.cap = a.c.max_blocks * a.c.block_size;
   kp.head_tiles = plan.head_tiles;
+  kp.unit_tiles = plan.unit_tiles;
+  kp.page = Divisor(a.c.block_size);
+  kp.least_units = plan.least_units;
   kp.group = a.q_heads / a.c.n_heads;
   if (a.weights_out) {
     kp.lse2 = reinterpret_cast<float *>(a.workspace + plan.lse2);

@@ -16,6 +16,24 @@ namespace kvs {
 // Element types of rows (KVS_DTYPE_* of kvs.h).
 enum : int32_t { kBf16 = 0, kFp16 = 1, kE4m3 = 2 };
 
+// Division of numbers below 2^31 by one divisor: a product and a shift. For l = ceil(log2 d) and
+// m = ceil(2^(31 + l) / d), m < 2^32 and floor(n m / 2^(31 + l)) = floor(n / d) for n < 2^31.
+struct Divisor {
+  uint32_t d, m, shift;
+  Divisor() = default;
+  explicit Divisor(uint32_t by) : d(by), m(0), shift(0) {
+    uint32_t l = 0;
+    while ((1ull << l) < by) ++l;
+    if (l == 0) return;  // by one: n itself
+    m = (uint32_t)(((1ull << (31 + l)) + by - 1) / by);
+    shift = l - 1;
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return d == 1 ? n : __umulhi(n, m) >> shift; }
+  __device__ __forceinline__ uint32_t rest(uint32_t n, uint32_t q) const { return n - q * d; }
+#endif
+};
+
 // A paged cache as the kernels address it: row (page, head, slot) of K starts at
 // k + page * k_page + head * k_head + slot * k_row (bytes), so any page layout with contiguous
 // rows works. Page-table entries <= 0 hold nothing, entries >= num_blocks are out of range.
