@@ -5,11 +5,13 @@
 // position), `keep` in all. Their rows move, in order, to slots 0, 1, ... of the destination.
 //
 // Choosing: weights become 32-bit keys that sort as the weights do (0: no token, the largest: a
-// token that stays), and the keep-th largest key is found by its digits of 8 bits, most significant
-// first: a histogram of the keys that share the digits found so far, then the bin in which the
-// count from above reaches what is left. A cluster of up to 8 CTAs shares a row; the keys stay in
-// shared memory between the passes, so the weights are read from memory once, and the CTAs read one
-// another's histograms there. Chosen tokens are ranked by counting from the row's start, so the
+// token that stays), and the keep-th largest key is found by its digits of 12, 10 and 10 bits, most
+// significant first: a histogram of the keys that share the digits found so far, then the bin in
+// which the count from above reaches what is left. (Twelve bits first: sign, exponent and three bits
+// more, so that weights of like size do not all count in a few bins.) A cluster of up to 8 CTAs
+// shares a row; the keys stay in shared memory between the passes, so the weights are read from memory
+// once, and the CTAs add up one another's histograms there. What bounds it is latency: three rounds of
+// counting, exchange and scan. Chosen tokens are ranked by counting from the row's start, so the
 // result does not depend on timing.
 //
 // Moving: to fresh pages, rows are copied by as many CTAs as there are rows for. In place, the rows
@@ -33,7 +35,7 @@ namespace cg = cooperative_groups;
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr uint32_t kStays = 0xFFFFFFFFu;
-constexpr uint32_t kMaxCached = 49152;  // keys a CTA holds in shared memory (192 KiB)
+constexpr uint32_t kMaxCached = 49152;  // keys a CTA holds in shared memory (192 KiB beside its histograms)
 
 // Keys sort as the weights: NaN above +inf, -0 equal to 0, never 0 and never kStays.
 __device__ __forceinline__ uint32_t key_of(float w) {
@@ -48,18 +50,87 @@ __device__ __forceinline__ uint32_t length_of(const EvictParams &p, uint32_t b) 
   return n <= 0 ? 0 : min((uint32_t)n, p.c.max_blocks * p.c.block_size);
 }
 
+constexpr uint32_t kBins[3] = {4096, 1024, 1024};
+constexpr uint32_t kAllBins = 4096 + 1024 + 1024;
+
+struct Found {
+  uint32_t bin, left, total;
+};
+
+// Adds up the cluster's histograms (`hist` in each CTA's shared memory), scans them from the largest
+// bin down and finds the one in which the count reaches `want` of all that was counted (`all`: of
+// min(total, want)). Same result in every CTA and thread; bin is BINS where everything is wanted.
+template <uint32_t BINS>
+__device__ Found find_bin(cg::cluster_group &cluster, uint32_t *hist, uint32_t want, uint32_t *s_warp, uint32_t *s_out) {
+  constexpr uint32_t per = BINS / kSelThreads;
+  static_assert(per == 2 || per == 8, "whole vectors per thread");
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t low = BINS - (tid + 1) * per;  // this thread's lowest bin
+  uint32_t bins[per];
+#pragma unroll
+  for (uint32_t i = 0; i < per; ++i) bins[i] = 0;
+  for (uint32_t r = 0; r < cluster.num_blocks(); ++r) {
+    const uint32_t *from = cluster.map_shared_rank(hist, r) + low;
+    if (per == 8) {
+#pragma unroll
+      for (uint32_t i = 0; i < per; i += 4) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(from + i);
+        bins[i] += x.x, bins[(i + 1) % per] += x.y, bins[(i + 2) % per] += x.z, bins[(i + 3) % per] += x.w;
+      }
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2 *>(from);
+      bins[0] += x.x, bins[1] += x.y;
+    }
+  }
+  uint32_t sum = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < per; ++i) sum += bins[i];
+  uint32_t incl = sum;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(~0u, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  __syncthreads();
+  uint32_t before = 0, total = 0;
+  for (uint32_t i = 0; i < kSelWarps; ++i) {
+    if (i < warp) before += s_warp[i];
+    total += s_warp[i];
+  }
+  incl += before;
+  const uint32_t goal = min(want, total);
+  if (tid == 0) {
+    s_out[0] = BINS;
+    s_out[1] = 0;
+  }
+  __syncthreads();
+  uint32_t above = incl - sum;
+  if (goal < total && above < goal && goal <= incl) {
+#pragma unroll
+    for (uint32_t i = per; i-- > 0;) {
+      if (above < goal && goal <= above + bins[i]) {
+        s_out[0] = low + i;
+        s_out[1] = goal - above;
+      }
+      above += bins[i];
+    }
+  }
+  __syncthreads();
+  return Found{s_out[0], s_out[1], total};
+}
+
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_constant__ EvictParams p, uint32_t cached_keys) {
-  extern __shared__ uint32_t s_keys[];
-  __shared__ uint32_t s_hist[4][256];
-  __shared__ uint32_t s_count[3];           // tokens, above the threshold, equal to it
+  extern __shared__ __align__(16) uint32_t s_keys[];
+  __shared__ __align__(16) uint32_t s_hist[kAllBins];
+  __shared__ uint32_t s_count[2];           // above the threshold, equal to it
   __shared__ uint32_t s_warp[2][kSelWarps];
-  __shared__ uint32_t s_bin[2];
+  __shared__ uint32_t s_out[2];
   cg::cluster_group cluster = cg::this_cluster();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const uint32_t row = blockIdx.x / ctas, b = row / p.c.n_heads, h = row % p.c.n_heads;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t len = length_of(p, b);
-  // this CTA's tokens: a piece of whole warps' shares
   const uint32_t piece = (len + ctas - 1) / ctas;
   const uint32_t t0 = min(len, rank * piece), n = min(len - t0, piece);
   const float *w = p.weights + (int64_t)b * p.w_req + (int64_t)h * p.w_head;
@@ -67,84 +138,69 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
 
   auto compute = [&](uint32_t i) -> uint32_t {
     const uint32_t t = t0 + i;
-    if (page_of(p.c, b, t / p.c.block_size) <= 0) return 0u;
-    if (t < p.first || t + p.recent >= len) return kStays;
-    return key_of(__ldg(w + t));
+    const float x = __ldg(w + t);
+    if (page_of(p.c, b, p.page.quotient(t)) <= 0) return 0u;
+    return t < p.first || t + p.recent >= len ? kStays : key_of(x);
   };
   auto key_at = [&](uint32_t i) -> uint32_t { return cached ? s_keys[i] : compute(i); };
 
-  for (uint32_t i = tid; i < 4 * 256; i += kSelThreads) (&s_hist[0][0])[i] = 0;
-  if (tid < 3) s_count[tid] = 0;
+  for (uint32_t i = tid; i < kAllBins; i += kSelThreads) s_hist[i] = 0;
   __syncthreads();
-  uint32_t there = 0;
-  for (uint32_t i = tid; i < n; i += kSelThreads) {
-    const uint32_t key = compute(i);
-    if (cached) s_keys[i] = key;
-    there += key != 0;
+  constexpr uint32_t kAhead = 8;
+  for (uint32_t base = tid; base < n; base += kSelThreads * kAhead) {
+    uint32_t key[kAhead];
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u) {
+      const uint32_t i = base + u * kSelThreads;
+      key[u] = i < n ? compute(i) : 0;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u) {
+      const uint32_t i = base + u * kSelThreads;
+      if (cached && i < n) s_keys[i] = key[u];
+      if (key[u]) atomicAdd(&s_hist[key[u] >> 20], 1u);
+    }
   }
-  for (int o = 16; o; o >>= 1) there += __shfl_xor_sync(~0u, there, o);
-  if (lane == 0 && there) atomicAdd(&s_count[0], there);
   cluster.sync();
-  uint32_t tokens = 0;
-  for (uint32_t r = 0; r < ctas; ++r) tokens += *cluster.map_shared_rank(&s_count[0], r);
-  const uint32_t want = min(tokens, p.keep);
-
-  uint32_t found = 0, mask = 0, left = want;  // digits found so far; ranks still wanted among equal ones
-  if (want < tokens && want > 0) {
-    for (int pass = 0; pass < 4; ++pass) {
-      const int shift = 24 - 8 * pass;
+  Found f = find_bin<4096>(cluster, s_hist, p.keep, s_warp[0], s_out);
+  const uint32_t want = min(f.total, p.keep);
+  uint32_t found = 1, left = 0xFFFFFFFFu;  // every token there is (keys are 1 or more)
+  if (f.bin < 4096) {
+    found = f.bin << 20;
+    for (uint32_t i = tid; i < n; i += kSelThreads) {
+      const uint32_t key = key_at(i);
+      if (key && key >> 20 == f.bin) atomicAdd(&s_hist[4096 + (key >> 10 & 1023)], 1u);
+    }
+    cluster.sync();
+    // where all of a bin is wanted, its lowest key is as good a threshold as any
+    Found g = find_bin<1024>(cluster, s_hist + 4096, f.left, s_warp[0], s_out);
+    left = g.left;
+    if (g.bin < 1024) {
+      found |= g.bin << 10;
       for (uint32_t i = tid; i < n; i += kSelThreads) {
         const uint32_t key = key_at(i);
-        if (key && (key & mask) == found) atomicAdd(&s_hist[pass][key >> shift & 255], 1u);
+        if (key && key >> 10 == found >> 10) atomicAdd(&s_hist[5120 + (key & 1023)], 1u);
       }
       cluster.sync();
-      if (warp == 0) {
-        // lane holds bins 255 - 8 lane, ... downwards
-        uint32_t bins[8], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t bin = 255 - 8 * lane - i;
-          bins[i] = 0;
-          for (uint32_t r = 0; r < ctas; ++r) bins[i] += *cluster.map_shared_rank(&s_hist[pass][bin], r);
-          sum += bins[i];
-        }
-        uint32_t incl = sum;
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t y = __shfl_up_sync(~0u, incl, o);
-          if (lane >= o) incl += y;
-        }
-        uint32_t above = incl - sum;
-        if (above < left && left <= incl) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (above < left && left <= above + bins[i]) {
-              s_bin[0] = 255 - 8 * lane - i;
-              s_bin[1] = left - above;
-            }
-            above += bins[i];
-          }
-        }
-      }
-      __syncthreads();
-      found |= s_bin[0] << shift;
-      mask |= 255u << shift;
-      left = s_bin[1];
-      __syncthreads();
+      g = find_bin<1024>(cluster, s_hist + 5120, g.left, s_warp[0], s_out);
+      left = g.left;
+      if (g.bin < 1024) found |= g.bin;
+      else left = 0xFFFFFFFFu;
+    } else {
+      left = 0xFFFFFFFFu;
     }
-  } else {
-    found = 1;  // every token there is, or none
-    left = want > 0 ? 0xFFFFFFFFu : 0;
+    found = max(found, 1u);
   }
   // chosen: keys above `found`, and the first `left` keys equal to it
   const uint32_t share = ((n + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
   const uint32_t i0 = min(n, warp * share), i1 = min(n, i0 + share);
   uint32_t above = 0, equal = 0;
-  if (want > 0)
-    for (uint32_t i = i0; i < i1; i += 32) {
-      const uint32_t key = i + lane < i1 ? key_at(i + lane) : 0;
-      above += __popc(__ballot_sync(~0u, key > found));
-      equal += __popc(__ballot_sync(~0u, key == found && key != 0));
-    }
+  for (uint32_t i = i0; i < i1; i += 32) {
+    const uint32_t key = i + lane < i1 ? key_at(i + lane) : 0;
+    above += __popc(__ballot_sync(~0u, key > found));
+    equal += __popc(__ballot_sync(~0u, key == found));
+  }
+  __syncthreads();  // s_warp is read no more
   if (lane == 0) {
     s_warp[0][warp] = above;
     s_warp[1][warp] = equal;
@@ -153,30 +209,28 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   if (tid < 2) {
     uint32_t sum = 0;
     for (int i = 0; i < kSelWarps; ++i) sum += s_warp[tid][i];
-    s_count[1 + tid] = sum;
+    s_count[tid] = sum;
   }
   cluster.sync();
   above = equal = 0;
   for (uint32_t r = 0; r < rank; ++r) {
-    above += *cluster.map_shared_rank(&s_count[1], r);
-    equal += *cluster.map_shared_rank(&s_count[2], r);
+    above += *cluster.map_shared_rank(&s_count[0], r);
+    equal += *cluster.map_shared_rank(&s_count[1], r);
   }
   for (uint32_t i = 0; i < warp; ++i) {
     above += s_warp[0][i];
     equal += s_warp[1][i];
   }
   int32_t *kept = p.kept + (uint64_t)row * p.keep;
-  if (want > 0)
-    for (uint32_t i = i0; i < i1; i += 32) {
-      const uint32_t key = i + lane < i1 ? key_at(i + lane) : 0;
-      const uint32_t ba = __ballot_sync(~0u, key > found), be = __ballot_sync(~0u, key == found && key != 0);
-      const uint32_t below = (1u << lane) - 1;
-      const uint32_t a = above + __popc(ba & below), e = equal + __popc(be & below);
-      const bool chosen = key > found || (key == found && key != 0 && e < left);
-      if (chosen) kept[a + min(e, left)] = (int32_t)(t0 + i + lane);
-      above += __popc(ba);
-      equal += __popc(be);
-    }
+  for (uint32_t i = i0; i < i1; i += 32) {
+    const uint32_t key = i + lane < i1 ? key_at(i + lane) : 0;
+    const uint32_t ba = __ballot_sync(~0u, key > found), be = __ballot_sync(~0u, key == found);
+    const uint32_t below = (1u << lane) - 1;
+    const uint32_t a = above + __popc(ba & below), e = equal + __popc(be & below);
+    if (key > found || (key == found && e < left)) kept[a + min(e, left)] = (int32_t)(t0 + i + lane);
+    above += __popc(ba);
+    equal += __popc(be);
+  }
   for (uint32_t i = want + rank * kSelThreads + tid; i < p.keep; i += ctas * kSelThreads) kept[i] = -1;
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = (int32_t)want;
   cluster.sync();  // no CTA leaves while another reads its counts
@@ -313,9 +367,10 @@ __global__ void __launch_bounds__(kMoveThreads) move_in_place_kernel(const __gri
 cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   if (p.c.batch == 0) return cudaSuccess;
   const uint64_t cap = (uint64_t)p.c.max_blocks * p.c.block_size;
-  // a row of up to 8192 tokens is one CTA's; longer ones are shared by a cluster
+  // CTAs per row: pieces of 1024 tokens while the GPU has room for more CTAs, of 8192 otherwise
+  const uint64_t rows = (uint64_t)p.c.batch * p.c.n_heads;
   uint32_t ctas = 1;
-  while (ctas < 8 && cap > 8192ull * ctas) ctas *= 2;
+  while (ctas < 8 && cap > 1024ull * ctas && (rows * ctas < 2ull * sms || cap > 8192ull * ctas)) ctas *= 2;
   const uint64_t piece = (cap + ctas - 1) / ctas;
   const uint32_t cached = piece <= kMaxCached ? (uint32_t)piece : 0;
   const size_t smem = 4ull * cached;

@@ -192,6 +192,7 @@ int kvs_qk_norm_rope_fill(const kvs_paged_cache *cache, const kvs_qkv_rows *r, v
   p.eps = r->eps;
   p.interleaved = r->interleaved;
   p.zero_rest = r->zero_rest;
+  p.page = kvs::Divisor(p.c.block_size);
   CUDA_TRY(kvs::launch_qkv_fill(p, static_cast<cudaStream_t>(stream)), op);
   return KVS_OK;
 }
@@ -295,6 +296,7 @@ int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *r, void 
   p.kept = r->kept;
   p.new_lens = r->new_lens;
   p.out_of_range = r->out_of_range;
+  p.page = kvs::Divisor(p.c.block_size);
   p.row_bytes = cache->head_dim * (cache->dtype == KVS_DTYPE_E4M3 ? 1 : 2);
   CUDA_TRY(kvs::launch_evict(p, sms, static_cast<cudaStream_t>(stream)), op);
   return KVS_OK;

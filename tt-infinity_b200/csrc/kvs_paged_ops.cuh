@@ -71,6 +71,7 @@ struct QkvFillParams {
   int32_t dtype;                // of q, k, v and q_out
   float eps;
   int interleaved, zero_rest;
+  Divisor page;                 // block_size
 };
 cudaError_t launch_qkv_fill(const QkvFillParams &p, cudaStream_t stream);
 
@@ -108,6 +109,7 @@ struct EvictParams {
   int32_t *new_lens;          // [batch]
   uint32_t *out_of_range;
   uint32_t row_bytes;
+  Divisor page;               // block_size
 };
 cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream);
 

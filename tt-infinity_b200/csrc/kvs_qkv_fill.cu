@@ -8,10 +8,13 @@
 // 32 bits, rounded once on the way out. Values are only copied (and scaled for an e4m3 cache).
 //
 // What bounds it: each row is read once and written once; a token step of a few tokens is bound by
-// the chain of lookups (request, start, page, cosines) ahead of the first row. A group of
-// head_dim / 8 lanes owns a row, each lane the same four pairs of every row: a pair's two elements
-// sit in one lane (two 8-byte accesses, or one of 16 bytes), so the rotation needs no exchange, the
-// norm one reduction, and cosines, sines and weights stay in registers over a token's rows.
+// the chain of lookups (request, start, page, cosines), which the first rows' loads do not wait for.
+// A warp takes one token and some of its rows of one kind (q, k or v). A few lanes own a row, each the
+// same pairs of every row: a pair's two elements sit in one lane, so the rotation needs no exchange and
+// the norm one reduction over the row's lanes. Norm weight, cosine and sine of a pair are four
+// coefficients that stay in registers over the warp's rows:
+//     (a, b) -> (a A + b B, a C + b D) / sqrt(mean + eps)    A = wa cos, B = -wb sin, C = wa sin, D = wb cos
+// and the next rows are loaded while these are computed.
 #include "kvs_paged_ops.cuh"
 
 #include <cuda_bf16.h>
@@ -24,8 +27,10 @@ namespace kvs {
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kUnroll = 4;  // rows in flight per lane
+#ifndef TUNE_U
+#define TUNE_U 2
+#endif
+constexpr int kUnroll = TUNE_U;  // rows in flight per lane
 
 template <bool kBf>
 __device__ __forceinline__ float2 widen2(uint32_t x) {
@@ -60,178 +65,304 @@ __device__ __forceinline__ uint32_t entries_up_to(const int32_t *cu, uint32_t n,
   return lo;
 }
 
-// kLanes lanes own a row. Each warp takes one token and `rows_per` of its rows.
-template <bool kBf, int kLanes>
-__global__ void __launch_bounds__(32 * kWarps) qkv_fill_kernel(const __grid_constant__ QkvFillParams p, uint32_t parts, uint32_t rows_per) {
-  constexpr uint32_t rows_at_once = 32 / kLanes;
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t item = (uint64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const uint32_t t = (uint32_t)(item / parts), part = (uint32_t)(item % parts);
-  if (t >= p.tokens) return;
+// PP pairs of 16-bit elements: half of a lane's elements of a row, one access.
+template <int PP>
+struct Half;
+template <>
+struct Half<4> {
+  using type = uint2;
+};
+template <>
+struct Half<8> {
+  using type = uint4;
+};
+
+// PP pairs per lane, kLanes lanes per row (32 / kLanes rows at once).
+template <bool kBf, bool kInter, int PP, int kLanes>
+struct Rows {
+  using H = typename Half<PP>::type;
+  static constexpr uint32_t at_once = 32 / kLanes;
+  static constexpr uint32_t step = kUnroll * at_once;
+
+  // Where the halves of this lane's pairs lie in a row, and whether the pairs are rotated.
+  struct Place {
+    uint32_t e0, e1, pair, sub;
+    bool mine, turns;
+  };
+  __device__ static __forceinline__ Place place(const QkvFillParams &p, uint32_t lane) {
+    Place w;
+    const uint32_t half = p.rotary / 2;
+    w.pair = PP * (lane % kLanes);
+    w.sub = lane / kLanes;
+    w.mine = 2 * w.pair < p.c.head_dim;
+    w.turns = w.pair < half;
+    w.e0 = kInter ? 2 * w.pair : (w.turns ? w.pair : w.pair + half);
+    w.e1 = kInter ? 2 * w.pair + PP : w.e0 + (w.turns ? half : (p.c.head_dim - p.rotary) / 2);
+    return w;
+  }
+  // a row's elements of this lane as first and second elements of its pairs
+  __device__ static __forceinline__ void split(const H &lo, const H &hi, float (&a)[PP], float (&b)[PP]) {
+    const uint32_t *x = reinterpret_cast<const uint32_t *>(&lo), *y = reinterpret_cast<const uint32_t *>(&hi);
+#pragma unroll
+    for (int i = 0; i < PP / 2; ++i) {
+      const float2 u = widen2<kBf>(x[i]), v = widen2<kBf>(y[i]);
+      if (kInter) {
+        a[i] = u.x, b[i] = u.y;
+        a[PP / 2 + i] = v.x, b[PP / 2 + i] = v.y;
+      } else {
+        a[2 * i] = u.x, a[2 * i + 1] = u.y;
+        b[2 * i] = v.x, b[2 * i + 1] = v.y;
+      }
+    }
+  }
+  // two halves in the order of memory
+  __device__ static __forceinline__ void unsplit(const float (&a)[PP], const float (&b)[PP], float (&x)[2 * PP]) {
+#pragma unroll
+    for (int i = 0; i < PP; ++i) {
+      x[i] = kInter ? (i & 1 ? b[i / 2] : a[i / 2]) : a[i];
+      x[PP + i] = kInter ? (i & 1 ? b[PP / 2 + i / 2] : a[PP / 2 + i / 2]) : b[i];
+    }
+  }
+  __device__ static __forceinline__ void store16(uint8_t *o, const Place &w, const float (&x)[2 * PP]) {
+    H h[2];
+    uint32_t *y = reinterpret_cast<uint32_t *>(h);
+#pragma unroll
+    for (int i = 0; i < PP; ++i) y[i] = narrow2<kBf>(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<H *>(o + 2 * w.e0) = h[0];
+    *reinterpret_cast<H *>(o + 2 * w.e1) = h[1];
+  }
+  __device__ static __forceinline__ void store8(uint8_t *o, const Place &w, const float (&x)[2 * PP], float f) {
+    uint32_t y[PP / 2];
+#pragma unroll
+    for (int i = 0; i < PP / 2; ++i) y[i] = narrow4_e4m3(x[4 * i] * f, x[4 * i + 1] * f, x[4 * i + 2] * f, x[4 * i + 3] * f);
+    if (PP == 8) {
+      *reinterpret_cast<uint2 *>(o + w.e0) = make_uint2(y[0], y[1]);
+      *reinterpret_cast<uint2 *>(o + w.e1) = make_uint2(y[PP / 4], y[PP / 4 + 1]);
+    } else {
+      *reinterpret_cast<uint32_t *>(o + w.e0) = y[0];
+      *reinterpret_cast<uint32_t *>(o + w.e1) = y[1];
+    }
+  }
+  // rows [row, row + step) below `end`, `stride` bytes apart
+  __device__ static __forceinline__ void load(const uint8_t *x, int64_t stride, uint32_t row, uint32_t end, const Place &w, H (&lo)[kUnroll], H (&hi)[kUnroll]) {
+    const uint8_t *at = x + (int64_t)(row + w.sub) * stride;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (row + u * at_once + w.sub < end && w.mine) {
+        lo[u] = *reinterpret_cast<const H *>(at + 2 * w.e0);
+        hi[u] = *reinterpret_cast<const H *>(at + 2 * w.e1);
+      }
+      at += at_once * stride;
+    }
+  }
+
+  // Norm and rotation of the rows [row, end) (the first `step` of them already loaded): `coef` as above.
+  template <bool k8>
+  __device__ static __forceinline__ void turn(const QkvFillParams &p, const Place &w, const uint8_t *x, int64_t in, uint8_t *o, int64_t out, uint32_t row,
+                                              uint32_t end, H (&lo)[kUnroll], H (&hi)[kUnroll], const float (&coef)[4][PP], bool normed, float scale) {
+    const float inv_dim = 1.f / (float)p.c.head_dim;
+    for (; row < end; row += step) {
+      H next_lo[kUnroll], next_hi[kUnroll];
+      load(x, in, row + step, end, w, next_lo, next_hi);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        float a[PP], b[PP], r[2 * PP];
+        split(lo[u], hi[u], a, b);
+        float f = 1.f;
+        if (normed) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < PP; ++i) ss += a[i] * a[i] + b[i] * b[i];
+          if (!w.mine) ss = 0.f;
+#pragma unroll
+          for (int k = kLanes / 2; k; k >>= 1) ss += __shfl_xor_sync(~0u, ss, k);
+          f = rsqrtf(ss * inv_dim + p.eps);
+        }
+        float y[PP], z[PP];
+#pragma unroll
+        for (int i = 0; i < PP; ++i) {
+          y[i] = a[i] * coef[0][i];
+          z[i] = b[i] * coef[3][i];
+          if (w.turns) {
+            y[i] += b[i] * coef[1][i];
+            z[i] += a[i] * coef[2][i];
+          }
+          y[i] *= f;
+          z[i] *= f;
+        }
+        const uint32_t q = row + u * at_once + w.sub;
+        if (q < end && w.mine) {
+          unsplit(y, z, r);
+          if (k8) store8(o + (int64_t)q * out, w, r, scale);
+          else store16(o + (int64_t)q * out, w, r);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        lo[u] = next_lo[u];
+        hi[u] = next_hi[u];
+      }
+    }
+  }
+};
+
+// Jobs of a token: q_parts warps for its queries, then warps for its keys and values, each `per` rows
+// (of both).
+template <bool kBf, bool kInter, int PP, int kLanes>
+__global__ void __launch_bounds__(32) qkv_fill_kernel(const __grid_constant__ QkvFillParams p, uint32_t q_parts, uint32_t per) {
+  using R = Rows<kBf, kInter, PP, kLanes>;
+  const uint32_t lane = threadIdx.x, t = blockIdx.x;
   const PagedCache &c = p.c;
-  const uint32_t rows = p.q_heads + 2 * c.n_heads;
-  const uint32_t r0 = part * rows_per, r1 = min(rows, r0 + rows_per);
-  const uint32_t l = lane % kLanes, sub = lane / kLanes;
-  const uint32_t pair = 4 * l, half = p.rotary / 2, rest = (c.head_dim - p.rotary) / 2;
-  const bool mine = 2 * pair < c.head_dim;
-  const bool turns = pair < half;
-  // the first elements of this lane's pairs, and how far the second ones are (halves layout)
-  const uint32_t e0 = p.interleaved ? 2 * pair : (turns ? pair : pair + half);
-  const uint32_t e1 = p.interleaved ? 2 * pair + 4 : (turns ? pair + half : pair + half + rest);
+  const bool is_q = blockIdx.y < q_parts;
+  const uint32_t row0 = (is_q ? blockIdx.y : blockIdx.y - q_parts) * per, end = min(is_q ? p.q_heads : c.n_heads, row0 + per);
+  const typename R::Place w = R::place(p, lane);
+  const uint8_t *x = is_q ? p.q + (int64_t)t * p.q_tok : p.k + (int64_t)t * p.k_tok;
+  const uint8_t *v = p.v + (int64_t)t * p.v_tok;
+  const int64_t in = is_q ? p.q_head : p.k_head;
+  typename R::H lo[kUnroll], hi[kUnroll], v_lo[kUnroll], v_hi[kUnroll];
+  // the first rows are on their way while the token's place is looked up
+  R::load(x, in, row0, end, w, lo, hi);
+  if (!is_q) R::load(v, p.v_head, row0, end, w, v_lo, v_hi);
 
   // ---- the token: its request, its slot in the cache and its position
   const uint32_t upto = entries_up_to(p.cu_seqlens, c.batch + 1, t, lane);
   const bool inside = upto >= 1 && upto <= c.batch && (uint32_t)__ldg(p.cu_seqlens + upto) != 0xFFFFFFFFu;
-  if (!inside) {  // behind the last sequence
-    if (p.zero_rest && mine)
-      for (uint32_t r = r0 + sub; r < min(r1, p.q_heads); r += rows_at_once) {
+  bool bad = false;
+  uint32_t slot = 0, pos = 0, vb = 0;
+  int32_t page = 0;
+  if (inside) {
+    const uint32_t req = upto - 1;
+    slot = t - (uint32_t)__ldg(p.cu_seqlens + req) + (uint32_t)__ldg(p.start + req);
+    vb = slot < 0x80000000u ? p.page.quotient(slot) : c.max_blocks;
+    page = page_of(c, req, vb);
+    pos = slot;
+    if (p.positions) pos = lane < p.n_axes ? (uint32_t)__ldg(p.positions + (uint64_t)lane * p.tokens + t) : 0;
+    bad = __any_sync(~0u, pos >= p.n_positions);
+    if ((bad || page < 0) && blockIdx.y == 0 && lane == 0 && p.out_of_range) atomicAdd(p.out_of_range, 1u);
+  }
+  if (is_q && (!inside || bad)) {
+    if ((bad || p.zero_rest) && w.mine)  // rows behind the last sequence stay as they are unless asked for
+      for (uint32_t r = row0 + w.sub; r < end; r += R::at_once) {
         uint8_t *o = p.q_out + (int64_t)t * p.o_tok + (int64_t)r * p.o_head;
-        *reinterpret_cast<uint2 *>(o + 2 * e0) = make_uint2(0, 0);
-        *reinterpret_cast<uint2 *>(o + 2 * e1) = make_uint2(0, 0);
+        *reinterpret_cast<typename R::H *>(o + 2 * w.e0) = typename R::H{};
+        *reinterpret_cast<typename R::H *>(o + 2 * w.e1) = typename R::H{};
       }
     return;
   }
-  const uint32_t req = upto - 1;
-  const uint32_t slot = t - (uint32_t)__ldg(p.cu_seqlens + req) + (uint32_t)__ldg(p.start + req);
-  const int32_t page = page_of(c, req, slot / c.block_size);
-  uint32_t pos = slot;
-  if (p.positions) pos = lane < p.n_axes ? (uint32_t)__ldg(p.positions + (uint64_t)lane * p.tokens + t) : 0;
-  const bool bad = __any_sync(~0u, pos >= p.n_positions);
-  if ((bad || page < 0) && part == 0 && lane == 0 && p.out_of_range) atomicAdd(p.out_of_range, 1u);
-  float cs[4], sn[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t at = pos;
-    if (p.positions) {
-      const uint32_t axis = p.axes && turns ? (uint32_t)__ldg(p.axes + pair + i) : 0u;
-      at = __shfl_sync(~0u, pos, min(axis, p.n_axes - 1));
-    }
-    cs[i] = 1.f;
-    sn[i] = 0.f;
-    if (turns && !bad) {
-      cs[i] = __ldg(p.cos_sin + (uint64_t)at * p.rotary + pair + i);
-      sn[i] = __ldg(p.cos_sin + (uint64_t)at * p.rotary + half + pair + i);
-    }
-  }
-  const int64_t k_at = (int64_t)page * c.k_page + (int64_t)(slot % c.block_size) * c.k_row;
-  const int64_t v_at = (int64_t)page * c.v_page + (int64_t)(slot % c.block_size) * c.v_row;
-  const bool store = page > 0 && !bad;
-  const float inv_dim = 1.f / (float)c.head_dim;
-  const float k_inv = 1.f / c.k_scale, v_inv = 1.f / c.v_scale;
+  if (!is_q && (!inside || bad || page <= 0)) return;
+  const uint32_t in_page = slot - vb * c.block_size;
 
-  // a row's eight elements of this lane as (first, second) elements of its pairs
-  auto split = [&](uint2 lo, uint2 hi, float (&a)[4], float (&b)[4]) {
-    const float2 x0 = widen2<kBf>(lo.x), x1 = widen2<kBf>(lo.y), x2 = widen2<kBf>(hi.x), x3 = widen2<kBf>(hi.y);
-    if (p.interleaved) {
-      a[0] = x0.x; b[0] = x0.y; a[1] = x1.x; b[1] = x1.y; a[2] = x2.x; b[2] = x2.y; a[3] = x3.x; b[3] = x3.y;
-    } else {
-      a[0] = x0.x; a[1] = x0.y; a[2] = x1.x; a[3] = x1.y; b[0] = x2.x; b[1] = x2.y; b[2] = x3.x; b[3] = x3.y;
-    }
-  };
-  auto weight_of = [&](const void *w, float (&a)[4], float (&b)[4]) {
-    if (!w || !mine) return;
-    const uint8_t *x = static_cast<const uint8_t *>(w);
-    split(__ldg(reinterpret_cast<const uint2 *>(x + 2 * e0)), __ldg(reinterpret_cast<const uint2 *>(x + 2 * e1)), a, b);
-  };
-  float qa[4] = {1.f, 1.f, 1.f, 1.f}, qb[4] = {1.f, 1.f, 1.f, 1.f}, ka[4] = {1.f, 1.f, 1.f, 1.f}, kb[4] = {1.f, 1.f, 1.f, 1.f};
-  weight_of(p.q_weight, qa, qb);
-  weight_of(p.k_weight, ka, kb);
-
-  for (uint32_t base = r0; base < r1; base += kUnroll * rows_at_once) {
-    uint2 lo[kUnroll], hi[kUnroll];
+  if (!is_q) {
+    uint8_t *o = c.v + (int64_t)page * c.v_page + (int64_t)in_page * c.v_row;
+    const float f = 1.f / c.v_scale;
+    for (uint32_t row = row0; row < end; row += R::step) {
+      if (row != row0) R::load(v, p.v_head, row, end, w, v_lo, v_hi);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint32_t r = base + u * rows_at_once + sub;
-      lo[u] = hi[u] = make_uint2(0, 0);
-      if (r < r1 && mine) {
-        const uint8_t *x = r < p.q_heads ? p.q + (int64_t)t * p.q_tok + (int64_t)r * p.q_head
-                           : r < p.q_heads + c.n_heads ? p.k + (int64_t)t * p.k_tok + (int64_t)(r - p.q_heads) * p.k_head
-                                                       : p.v + (int64_t)t * p.v_tok + (int64_t)(r - p.q_heads - c.n_heads) * p.v_head;
-        lo[u] = *reinterpret_cast<const uint2 *>(x + 2 * e0);
-        hi[u] = *reinterpret_cast<const uint2 *>(x + 2 * e1);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint32_t r = base + u * rows_at_once + sub;
-      const bool is_q = r < p.q_heads, is_k = !is_q && r < p.q_heads + c.n_heads;
-      float a[4], b[4];
-      split(lo[u], hi[u], a, b);
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ss += a[i] * a[i] + b[i] * b[i];
-#pragma unroll
-      for (int o = kLanes / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
-      if (is_q || is_k) {
-        const bool normed = is_q ? p.q_weight != nullptr : p.k_weight != nullptr;
-        const float f = normed ? rsqrtf(ss * inv_dim + p.eps) : 1.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = a[i] * f * (is_q ? qa[i] : ka[i]), y = b[i] * f * (is_q ? qb[i] : kb[i]);
-          a[i] = turns ? x * cs[i] - y * sn[i] : x;
-          b[i] = turns ? x * sn[i] + y * cs[i] : y;
-        }
-      }
-      if (r >= r1 || !mine) continue;
-      uint8_t *o;
-      if (is_q) {
-        o = p.q_out + (int64_t)t * p.o_tok + (int64_t)r * p.o_head;
-        if (bad) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] = b[i] = 0.f;
-        }
-      } else {
-        if (!store) continue;
-        o = is_k ? c.k + k_at + (int64_t)(r - p.q_heads) * c.k_head : c.v + v_at + (int64_t)(r - p.q_heads - c.n_heads) * c.v_head;
+      for (int u = 0; u < kUnroll; ++u) {
+        const uint32_t r = row + u * R::at_once + w.sub;
+        if (r >= end || !w.mine) continue;
+        uint8_t *to = o + (int64_t)r * c.v_head;
         if (c.dtype == kE4m3) {
-          const float f = is_k ? k_inv : v_inv;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            a[i] *= f;
-            b[i] *= f;
-          }
-          if (p.interleaved) {
-            *reinterpret_cast<uint32_t *>(o + e0) = narrow4_e4m3(a[0], b[0], a[1], b[1]);
-            *reinterpret_cast<uint32_t *>(o + e1) = narrow4_e4m3(a[2], b[2], a[3], b[3]);
-          } else {
-            *reinterpret_cast<uint32_t *>(o + e0) = narrow4_e4m3(a[0], a[1], a[2], a[3]);
-            *reinterpret_cast<uint32_t *>(o + e1) = narrow4_e4m3(b[0], b[1], b[2], b[3]);
-          }
-          continue;
+          float a[PP], b[PP], y[2 * PP];
+          R::split(v_lo[u], v_hi[u], a, b);
+          R::unsplit(a, b, y);
+          R::store8(to, w, y, f);
+        } else {
+          *reinterpret_cast<typename R::H *>(to + 2 * w.e0) = v_lo[u];
+          *reinterpret_cast<typename R::H *>(to + 2 * w.e1) = v_hi[u];
         }
-      }
-      if (p.interleaved) {
-        *reinterpret_cast<uint2 *>(o + 2 * e0) = make_uint2(narrow2<kBf>(a[0], b[0]), narrow2<kBf>(a[1], b[1]));
-        *reinterpret_cast<uint2 *>(o + 2 * e1) = make_uint2(narrow2<kBf>(a[2], b[2]), narrow2<kBf>(a[3], b[3]));
-      } else {
-        *reinterpret_cast<uint2 *>(o + 2 * e0) = make_uint2(narrow2<kBf>(a[0], a[1]), narrow2<kBf>(a[2], a[3]));
-        *reinterpret_cast<uint2 *>(o + 2 * e1) = make_uint2(narrow2<kBf>(b[0], b[1]), narrow2<kBf>(b[2], b[3]));
       }
     }
   }
+
+  // ---- coefficients of this lane's pairs
+  float coef[4][PP];
+  const void *weight = is_q ? p.q_weight : p.k_weight;
+  float wa[PP], wb[PP];
+#pragma unroll
+  for (int i = 0; i < PP; ++i) wa[i] = wb[i] = 1.f;
+  if (weight && w.mine)
+    R::split(__ldg(reinterpret_cast<const typename R::H *>(static_cast<const uint8_t *>(weight) + 2 * w.e0)),
+             __ldg(reinterpret_cast<const typename R::H *>(static_cast<const uint8_t *>(weight) + 2 * w.e1)), wa, wb);
+  const uint32_t half = p.rotary / 2;
+#pragma unroll
+  for (int i = 0; i < PP; i += 4) {
+    float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.axes) {
+      const int4 axis = w.turns ? __ldg(reinterpret_cast<const int4 *>(p.axes + w.pair + i)) : make_int4(0, 0, 0, 0);
+      const uint32_t of[4] = {(uint32_t)axis.x, (uint32_t)axis.y, (uint32_t)axis.z, (uint32_t)axis.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t at = __shfl_sync(~0u, pos, min(of[k], p.n_axes - 1));
+        if (w.turns) {
+          (&cs.x)[k] = __ldg(p.cos_sin + (uint64_t)at * p.rotary + w.pair + i + k);
+          (&sn.x)[k] = __ldg(p.cos_sin + (uint64_t)at * p.rotary + half + w.pair + i + k);
+        }
+      }
+    } else {
+      const uint32_t at = p.positions ? __shfl_sync(~0u, pos, 0) : pos;
+      if (w.turns) {
+        cs = __ldg(reinterpret_cast<const float4 *>(p.cos_sin + (uint64_t)at * p.rotary + w.pair + i));
+        sn = __ldg(reinterpret_cast<const float4 *>(p.cos_sin + (uint64_t)at * p.rotary + half + w.pair + i));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      // the pairs of an interleaved lane come as (first half, second half) of its elements: in order
+      coef[0][i + k] = wa[i + k] * (&cs.x)[k];
+      coef[1][i + k] = -wb[i + k] * (&sn.x)[k];
+      coef[2][i + k] = wa[i + k] * (&sn.x)[k];
+      coef[3][i + k] = wb[i + k] * (&cs.x)[k];
+    }
+  }
+  const bool normed = weight != nullptr;
+  if (is_q)
+    R::template turn<false>(p, w, x, in, p.q_out + (int64_t)t * p.o_tok, p.o_head, row0, end, lo, hi, coef, normed, 1.f);
+  else {
+    uint8_t *o = c.k + (int64_t)page * c.k_page + (int64_t)in_page * c.k_row;
+    if (c.dtype == kE4m3) R::template turn<true>(p, w, x, in, o, c.k_head, row0, end, lo, hi, coef, normed, 1.f / c.k_scale);
+    else R::template turn<false>(p, w, x, in, o, c.k_head, row0, end, lo, hi, coef, normed, 1.f);
+  }
+}
+
+template <bool kBf, bool kInter, int PP, int kLanes>
+cudaError_t run(const QkvFillParams &p, cudaStream_t stream) {
+  using R = Rows<kBf, kInter, PP, kLanes>;
+#ifndef TUNE_STEPS
+#define TUNE_STEPS 8
+#endif
+  // rows per warp: as many as leave enough warps
+  const uint32_t steps = (p.q_heads + R::step - 1) / R::step;
+  uint32_t per = TUNE_STEPS;
+  while (per > 1 && (uint64_t)p.tokens * ((steps + per - 1) / per) < 148 * 16) per /= 2;
+  const uint32_t q_parts = (steps + per - 1) / per, kv_parts = (p.c.n_heads + per * R::step - 1) / (per * R::step);
+  const dim3 grid(p.tokens, q_parts + kv_parts);
+  if (grid.y > 65535) return cudaErrorInvalidValue;
+  qkv_fill_kernel<kBf, kInter, PP, kLanes><<<grid, 32, 0, stream>>>(p, q_parts, per * R::step);
+  count_launch();
+  return cudaGetLastError();
+}
+
+template <bool kBf, bool kInter>
+cudaError_t run_dim(const QkvFillParams &p, cudaStream_t stream) {
+  const uint32_t d = p.c.head_dim;
+  // 16-byte halves where both the rotated part and the rest split into eights of pairs
+  if (p.rotary % 16 == 0 && d % 16 == 0) {
+    if (d <= 64) return run<kBf, kInter, 8, 4>(p, stream);
+    if (d <= 128) return run<kBf, kInter, 8, 8>(p, stream);
+    return run<kBf, kInter, 8, 16>(p, stream);
+  }
+  if (d <= 64) return run<kBf, kInter, 4, 8>(p, stream);
+  if (d <= 128) return run<kBf, kInter, 4, 16>(p, stream);
+  return run<kBf, kInter, 4, 32>(p, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_qkv_fill(const QkvFillParams &p, cudaStream_t stream) {
   if (p.tokens == 0) return cudaSuccess;
-  const uint32_t rows = p.q_heads + 2 * p.c.n_heads;
-  const int lanes = p.c.head_dim <= 64 ? 8 : (p.c.head_dim <= 128 ? 16 : 32);
-  const uint32_t step = kUnroll * (32 / lanes);
-  const uint32_t parts = (rows + step - 1) / step;
-  const uint64_t items = (uint64_t)p.tokens * parts;
-  const dim3 grid((unsigned)((items + kWarps - 1) / kWarps));
-  const bool bf = p.dtype == kBf16;
-#define KVS_FILL(kBf, kLanes) qkv_fill_kernel<kBf, kLanes><<<grid, 32 * kWarps, 0, stream>>>(p, parts, step)
-  if (bf && lanes == 8) KVS_FILL(true, 8);
-  else if (bf && lanes == 16) KVS_FILL(true, 16);
-  else if (bf) KVS_FILL(true, 32);
-  else if (lanes == 8) KVS_FILL(false, 8);
-  else if (lanes == 16) KVS_FILL(false, 16);
-  else KVS_FILL(false, 32);
-#undef KVS_FILL
-  count_launch();
-  return cudaGetLastError();
+  if (p.interleaved) return p.dtype == kBf16 ? run_dim<true, true>(p, stream) : run_dim<false, true>(p, stream);
+  return p.dtype == kBf16 ? run_dim<true, false>(p, stream) : run_dim<false, false>(p, stream);
 }
 
 }  // namespace kvs
