@@ -5,19 +5,20 @@
 // position), `keep` in all. Their rows move, in order, to slots 0, 1, ... of the destination.
 //
 // Choosing: weights become 32-bit keys that sort as the weights do (0: no token, the largest: a
-// token that stays), and the keep-th largest key is found by its digits of 12, 10 and 10 bits, most
+// token that stays), and the keep-th largest key is found by its digits of 10, 8, 8 and 6 bits, most
 // significant first: a histogram of the keys that share the digits found so far, then the bin in
-// which the count from above reaches what is left. (Twelve bits first: sign, exponent and three bits
-// more, so that weights of like size do not all count in a few bins.) A cluster of up to 8 CTAs
-// shares a row; the keys stay in shared memory between the passes, so the weights are read from memory
-// once, and the CTAs add up one another's histograms there. What bounds it is latency: three rounds of
-// counting, exchange and scan. Chosen tokens are ranked by counting from the row's start, so the
-// result does not depend on timing.
+// which the count from above reaches what is left. A cluster of up to 8 CTAs shares a row; the keys
+// stay in shared memory between the passes, so the weights are read from memory once, and the CTAs add
+// up one another's histograms there (digits of 12, 10 and 10 bits took longer: the exchange grows with
+// the bins). What bounds it is latency: four rounds of counting, exchange and scan, about 9 us for a
+// row of 4200 tokens. Chosen tokens are ranked by counting from the row's start, so the result does
+// not depend on timing.
 //
-// Moving: to fresh pages, rows are copied by as many CTAs as there are rows for. In place, the rows
-// of one (request, head) are moved by one CTA per 64-byte column of K or V, a batch of ranks at a
-// time: a kept token's rank is at most its position, so writing ranks [i, i + n) only overwrites
-// positions whose own rows have been read by then.
+// Moving: to fresh pages, each CTA moves the rows it chose of its tokens, in the same launch. In place,
+// a second kernel moves the rows of one (request, head) by one CTA per 64-byte column of K or V, a
+// batch of ranks at a time: a kept token's rank is at most its position, so writing ranks [i, i + n)
+// only overwrites positions whose own rows have been read by then. 12 prompts of up to 32768 tokens, 8
+// heads, trimmed to 4096: 92 us, of which the rows' 370 MB take 57 us at the measured copy rate.
 #include "kvs_paged_ops.cuh"
 
 #include <cooperative_groups.h>
@@ -32,7 +33,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr uint32_t kStays = 0xFFFFFFFFu;
 constexpr uint32_t kMaxCached = 49152;  // keys a CTA holds in shared memory (192 KiB beside its histograms)
@@ -50,38 +51,52 @@ __device__ __forceinline__ uint32_t length_of(const EvictParams &p, uint32_t b) 
   return n <= 0 ? 0 : min((uint32_t)n, p.c.max_blocks * p.c.block_size);
 }
 
-constexpr uint32_t kBins[3] = {4096, 1024, 1024};
-constexpr uint32_t kAllBins = 4096 + 1024 + 1024;
+// digits of the keys, most significant first: 10, 8, 8 and 6 bits
+constexpr uint32_t kAllBins = 1024 + 256 + 256 + 64;
+constexpr uint32_t kNoBin = 0xFFFFFFFFu;
 
 struct Found {
   uint32_t bin, left, total;
 };
 
+// Exclusive prefix of `mine` over the threads' warps (what the warps before this one hold) and the sum
+// over all: `mine` is the warp's total, the same in every lane.
+__device__ __forceinline__ uint2 over_warps(uint32_t mine, uint32_t *s_warp) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane == 0) s_warp[warp] = mine;
+  __syncthreads();
+  const uint32_t x = lane < kSelWarps ? s_warp[lane] : 0;
+  return make_uint2(__reduce_add_sync(~0u, lane < warp ? x : 0), __reduce_add_sync(~0u, x));
+}
+
 // Adds up the cluster's histograms (`hist` in each CTA's shared memory), scans them from the largest
-// bin down and finds the one in which the count reaches `want` of all that was counted (`all`: of
-// min(total, want)). Same result in every CTA and thread; bin is BINS where everything is wanted.
+// bin down and finds the one in which the count reaches min(want, total). Same result in every CTA and
+// thread; bin stays kNoBin where everything is wanted.
 template <uint32_t BINS>
 __device__ Found find_bin(cg::cluster_group &cluster, uint32_t *hist, uint32_t want, uint32_t *s_warp, uint32_t *s_out) {
-  constexpr uint32_t per = BINS / kSelThreads;
-  static_assert(per == 2 || per == 8, "whole vectors per thread");
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr uint32_t per = BINS <= kSelThreads ? 1 : BINS / kSelThreads;
+  static_assert(per == 1 || per == 2 || per == 4, "one access per thread");
+  const uint32_t tid = threadIdx.x, lane = tid & 31;
   const uint32_t low = BINS - (tid + 1) * per;  // this thread's lowest bin
-  uint32_t bins[per];
-#pragma unroll
-  for (uint32_t i = 0; i < per; ++i) bins[i] = 0;
-  for (uint32_t r = 0; r < cluster.num_blocks(); ++r) {
-    const uint32_t *from = cluster.map_shared_rank(hist, r) + low;
-    if (per == 8) {
-#pragma unroll
-      for (uint32_t i = 0; i < per; i += 4) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(from + i);
-        bins[i] += x.x, bins[(i + 1) % per] += x.y, bins[(i + 2) % per] += x.z, bins[(i + 3) % per] += x.w;
-      }
+  const uint32_t ctas = cluster.num_blocks();
+  uint32_t bins[per] = {};
+  auto add = [&](const uint32_t *from) {
+    if (per == 4) {
+      const uint4 x = *reinterpret_cast<const uint4 *>(from + low);
+      bins[0] += x.x, bins[1 % per] += x.y, bins[2 % per] += x.z, bins[3 % per] += x.w;
+    } else if (per == 2) {
+      const uint2 x = *reinterpret_cast<const uint2 *>(from + low);
+      bins[0] += x.x, bins[1 % per] += x.y;
     } else {
-      const uint2 x = *reinterpret_cast<const uint2 *>(from);
-      bins[0] += x.x, bins[1] += x.y;
+      bins[0] += from[low];
     }
-  }
+  };
+  const bool mine = tid * per < BINS;
+  if (mine) add(hist);
+  const uint32_t me = cluster.block_rank();
+#pragma unroll
+  for (uint32_t r = 1; r < 8; ++r)
+    if (r < ctas && mine) add(cluster.map_shared_rank(hist, (me + r) & (ctas - 1)));
   uint32_t sum = 0;
 #pragma unroll
   for (uint32_t i = 0; i < per; ++i) sum += bins[i];
@@ -90,22 +105,11 @@ __device__ Found find_bin(cg::cluster_group &cluster, uint32_t *hist, uint32_t w
     const uint32_t y = __shfl_up_sync(~0u, incl, o);
     if (lane >= o) incl += y;
   }
-  if (lane == 31) s_warp[warp] = incl;
-  __syncthreads();
-  uint32_t before = 0, total = 0;
-  for (uint32_t i = 0; i < kSelWarps; ++i) {
-    if (i < warp) before += s_warp[i];
-    total += s_warp[i];
-  }
-  incl += before;
-  const uint32_t goal = min(want, total);
-  if (tid == 0) {
-    s_out[0] = BINS;
-    s_out[1] = 0;
-  }
-  __syncthreads();
+  const uint2 w = over_warps(__shfl_sync(~0u, incl, 31), s_warp);
+  incl += w.x;
+  const uint32_t goal = min(want, w.y);
   uint32_t above = incl - sum;
-  if (goal < total && above < goal && goal <= incl) {
+  if (goal < w.y && above < goal && goal <= incl) {
 #pragma unroll
     for (uint32_t i = per; i-- > 0;) {
       if (above < goal && goal <= above + bins[i]) {
@@ -116,15 +120,72 @@ __device__ Found find_bin(cg::cluster_group &cluster, uint32_t *hist, uint32_t w
     }
   }
   __syncthreads();
-  return Found{s_out[0], s_out[1], total};
+  return Found{s_out[0], s_out[1], w.y};
 }
 
+// Page of slot i of request b's destination, or -1.
+__device__ __forceinline__ int32_t dst_page(const EvictParams &p, uint32_t b, uint32_t vb) {
+  if (vb >= p.dst_blocks) return -1;
+  const int32_t pg = __ldg(p.dst_table + (uint64_t)b * p.dst_blocks + vb);
+  return pg > 0 && (uint32_t)pg < p.c.num_blocks ? pg : -1;
+}
+
+// Where a batch of kept rows comes from and goes to, as byte offsets into K and V; -1: nowhere.
+constexpr uint32_t kMoveRows = 128;
+struct MoveRows {
+  int64_t k_src[kMoveRows], v_src[kMoveRows], k_dst[kMoveRows], v_dst[kMoveRows];
+};
+
+// Rows of the kept tokens of ranks [begin, end) to their slots on fresh pages, by the whole CTA.
+__device__ void move_rows(const EvictParams &p, uint32_t b, uint32_t h, const int32_t *kept, uint32_t begin, uint32_t end, MoveRows &s) {
+  const uint32_t tid = threadIdx.x, words = p.row_bytes / 16;
+  for (uint32_t base = begin; base < end; base += kMoveRows) {
+    const uint32_t rows = min(kMoveRows, end - base);
+    __syncthreads();
+    for (uint32_t r = tid; r < rows; r += kSelThreads) {
+      const uint32_t i = base + r, t = (uint32_t)kept[i];
+      const uint32_t sb = p.page.quotient(t), db = p.page.quotient(i), sr = p.page.rest(t, sb), dr = p.page.rest(i, db);
+      const int32_t sp = page_of(p.c, b, sb), dp = dst_page(p, b, db);
+      s.k_src[r] = (int64_t)sp * p.c.k_page + (int64_t)h * p.c.k_head + (int64_t)sr * p.c.k_row;
+      s.v_src[r] = (int64_t)sp * p.c.v_page + (int64_t)h * p.c.v_head + (int64_t)sr * p.c.v_row;
+      s.k_dst[r] = dp < 0 ? -1 : (int64_t)dp * p.c.k_page + (int64_t)h * p.c.k_head + (int64_t)dr * p.c.k_row;
+      s.v_dst[r] = dp < 0 ? -1 : (int64_t)dp * p.c.v_page + (int64_t)h * p.c.v_head + (int64_t)dr * p.c.v_row;
+      if (dp < 0 && h == 0 && p.out_of_range) atomicAdd(p.out_of_range, 1u);
+    }
+    __syncthreads();
+    const uint32_t side = rows * words;
+    constexpr int kAhead = 4;  // rows' words in flight per thread, of K and of V
+    for (uint32_t at = tid; at < side; at += kSelThreads * kAhead) {
+      int4 x[kAhead], y[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const uint32_t e = at + u * kSelThreads, r = p.words.quotient(e), q = p.words.rest(e, r);
+        if (e < side) {
+          x[u] = *reinterpret_cast<const int4 *>(p.c.k + s.k_src[r] + 16 * q);
+          y[u] = *reinterpret_cast<const int4 *>(p.c.v + s.v_src[r] + 16 * q);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const uint32_t e = at + u * kSelThreads, r = p.words.quotient(e), q = p.words.rest(e, r);
+        if (e < side && s.k_dst[r] >= 0) {
+          *reinterpret_cast<int4 *>(p.c.k + s.k_dst[r] + 16 * q) = x[u];
+          *reinterpret_cast<int4 *>(p.c.v + s.v_dst[r] + 16 * q) = y[u];
+        }
+      }
+    }
+  }
+}
+
+// Chooses the tokens of one (request, KV head) per cluster and moves what a CTA chose of its tokens:
+// their weights, and their rows where they go to fresh pages.
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_constant__ EvictParams p, uint32_t cached_keys) {
   extern __shared__ __align__(16) uint32_t s_keys[];
   __shared__ __align__(16) uint32_t s_hist[kAllBins];
   __shared__ uint32_t s_count[2];           // above the threshold, equal to it
-  __shared__ uint32_t s_warp[2][kSelWarps];
-  __shared__ uint32_t s_out[2];
+  __shared__ uint32_t s_warp[6][kSelWarps];
+  __shared__ uint32_t s_out[4][2];
+  __shared__ MoveRows s_rows;
   cg::cluster_group cluster = cg::this_cluster();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
@@ -136,61 +197,69 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   const float *w = p.weights + (int64_t)b * p.w_req + (int64_t)h * p.w_head;
   const bool cached = piece <= cached_keys;
 
-  auto compute = [&](uint32_t i) -> uint32_t {
-    const uint32_t t = t0 + i;
-    const float x = __ldg(w + t);
-    if (page_of(p.c, b, p.page.quotient(t)) <= 0) return 0u;
-    return t < p.first || t + p.recent >= len ? kStays : key_of(x);
+  // key of this CTA's token i from its weight and its page-table entry
+  const int32_t *table = p.c.page_table + (uint64_t)b * p.c.max_blocks;
+  auto key_from = [&](uint32_t i, float x, int32_t page) -> uint32_t {
+    const uint32_t t = t0 + i, key = t < p.first || t + p.recent >= len ? kStays : key_of(x);
+    return page > 0 && (uint32_t)page < p.c.num_blocks ? key : 0u;
   };
-  auto key_at = [&](uint32_t i) -> uint32_t { return cached ? s_keys[i] : compute(i); };
+  auto key_at = [&](uint32_t i) -> uint32_t { return cached ? s_keys[i] : key_from(i, __ldg(w + t0 + i), __ldg(table + p.page.quotient(t0 + i))); };
 
   for (uint32_t i = tid; i < kAllBins; i += kSelThreads) s_hist[i] = 0;
+  if (tid < 4) s_out[tid][0] = kNoBin;
   __syncthreads();
   constexpr uint32_t kAhead = 8;
   for (uint32_t base = tid; base < n; base += kSelThreads * kAhead) {
-    uint32_t key[kAhead];
+    float x[kAhead];
+    int32_t page[kAhead];
 #pragma unroll
-    for (uint32_t u = 0; u < kAhead; ++u) {
-      const uint32_t i = base + u * kSelThreads;
-      key[u] = i < n ? compute(i) : 0;
+    for (uint32_t u = 0; u < kAhead; ++u) {  // all on their way before the first is looked at
+      const uint32_t t = t0 + min(base + u * kSelThreads, n - 1);
+      x[u] = __ldg(w + t);
+      page[u] = __ldg(table + p.page.quotient(t));
     }
 #pragma unroll
     for (uint32_t u = 0; u < kAhead; ++u) {
       const uint32_t i = base + u * kSelThreads;
-      if (cached && i < n) s_keys[i] = key[u];
-      if (key[u]) atomicAdd(&s_hist[key[u] >> 20], 1u);
+      if (i >= n) break;
+      const uint32_t key = key_from(i, x[u], page[u]);
+      if (cached) s_keys[i] = key;
+      if (key) atomicAdd(&s_hist[key >> 22], 1u);
     }
   }
   cluster.sync();
-  Found f = find_bin<4096>(cluster, s_hist, p.keep, s_warp[0], s_out);
+  Found f = find_bin<1024>(cluster, s_hist, p.keep, s_warp[0], s_out[0]);
   const uint32_t want = min(f.total, p.keep);
-  uint32_t found = 1, left = 0xFFFFFFFFu;  // every token there is (keys are 1 or more)
-  if (f.bin < 4096) {
-    found = f.bin << 20;
+  // keys above `found` are chosen, and the first `left` equal to it; where all keys of a bin are
+  // wanted, its lowest key is as good a threshold as any (and with no bin at all the lowest key, 1)
+  uint32_t found = 0, left = kNoBin;
+  auto next_digit = [&](uint32_t *hist, uint32_t shift, uint32_t bits) {
     for (uint32_t i = tid; i < n; i += kSelThreads) {
       const uint32_t key = key_at(i);
-      if (key && key >> 20 == f.bin) atomicAdd(&s_hist[4096 + (key >> 10 & 1023)], 1u);
+      if (key && (key ^ found) >> (shift + bits) == 0) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
     }
     cluster.sync();
-    // where all of a bin is wanted, its lowest key is as good a threshold as any
-    Found g = find_bin<1024>(cluster, s_hist + 4096, f.left, s_warp[0], s_out);
-    left = g.left;
-    if (g.bin < 1024) {
-      found |= g.bin << 10;
-      for (uint32_t i = tid; i < n; i += kSelThreads) {
-        const uint32_t key = key_at(i);
-        if (key && key >> 10 == found >> 10) atomicAdd(&s_hist[5120 + (key & 1023)], 1u);
+  };
+  if (f.bin != kNoBin) {
+    found = f.bin << 22;
+    next_digit(s_hist + 1024, 14, 8);
+    f = find_bin<256>(cluster, s_hist + 1024, f.left, s_warp[1], s_out[1]);
+    if (f.bin != kNoBin) {
+      found |= f.bin << 14;
+      next_digit(s_hist + 1280, 6, 8);
+      f = find_bin<256>(cluster, s_hist + 1280, f.left, s_warp[2], s_out[2]);
+      if (f.bin != kNoBin) {
+        found |= f.bin << 6;
+        next_digit(s_hist + 1536, 0, 6);
+        f = find_bin<64>(cluster, s_hist + 1536, f.left, s_warp[3], s_out[3]);
+        if (f.bin != kNoBin) {
+          found |= f.bin;
+          left = f.left;
+        }
       }
-      cluster.sync();
-      g = find_bin<1024>(cluster, s_hist + 5120, g.left, s_warp[0], s_out);
-      left = g.left;
-      if (g.bin < 1024) found |= g.bin;
-      else left = 0xFFFFFFFFu;
-    } else {
-      left = 0xFFFFFFFFu;
     }
-    found = max(found, 1u);
   }
+  found = max(found, 1u);
   // chosen: keys above `found`, and the first `left` keys equal to it
   const uint32_t share = ((n + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
   const uint32_t i0 = min(n, warp * share), i1 = min(n, i0 + share);
@@ -200,27 +269,22 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     above += __popc(__ballot_sync(~0u, key > found));
     equal += __popc(__ballot_sync(~0u, key == found));
   }
-  __syncthreads();  // s_warp is read no more
-  if (lane == 0) {
-    s_warp[0][warp] = above;
-    s_warp[1][warp] = equal;
+  const uint2 of_above = over_warps(above, s_warp[4]), of_equal = over_warps(equal, s_warp[5]);
+  uint32_t cta_above = 0, cta_equal = 0;  // in the CTAs before this one
+  if (ctas > 1) {
+    if (tid == 0) {
+      s_count[0] = of_above.y;
+      s_count[1] = of_equal.y;
+    }
+    cluster.sync();
+    // lane r: the counts of CTA r, where it comes before this one
+    const bool before = lane < rank;
+    const uint32_t a = before ? *cluster.map_shared_rank(&s_count[0], lane) : 0, e = before ? *cluster.map_shared_rank(&s_count[1], lane) : 0;
+    cta_above = __reduce_add_sync(~0u, a);
+    cta_equal = __reduce_add_sync(~0u, e);
   }
-  __syncthreads();
-  if (tid < 2) {
-    uint32_t sum = 0;
-    for (int i = 0; i < kSelWarps; ++i) sum += s_warp[tid][i];
-    s_count[tid] = sum;
-  }
-  cluster.sync();
-  above = equal = 0;
-  for (uint32_t r = 0; r < rank; ++r) {
-    above += *cluster.map_shared_rank(&s_count[0], r);
-    equal += *cluster.map_shared_rank(&s_count[1], r);
-  }
-  for (uint32_t i = 0; i < warp; ++i) {
-    above += s_warp[0][i];
-    equal += s_warp[1][i];
-  }
+  above = cta_above + of_above.x;
+  equal = cta_equal + of_equal.x;
   int32_t *kept = p.kept + (uint64_t)row * p.keep;
   for (uint32_t i = i0; i < i1; i += 32) {
     const uint32_t key = i + lane < i1 ? key_at(i + lane) : 0;
@@ -233,16 +297,29 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   }
   for (uint32_t i = want + rank * kSelThreads + tid; i < p.keep; i += ctas * kSelThreads) kept[i] = -1;
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = (int32_t)want;
-  cluster.sync();  // no CTA leaves while another reads its counts
+  // the ranks of this CTA's tokens
+  const uint32_t begin = cta_above + min(cta_equal, left), end = cta_above + of_above.y + min(cta_equal + of_equal.y, left);
+  float *w_out = p.weights_out + (int64_t)b * p.wo_req + (int64_t)h * p.wo_head;
+  const bool in_turn = w_out == w;  // then every weight of the row is read before one is written
+  __syncthreads();
+  if (in_turn && cached)
+    for (uint32_t i = begin + tid; i < end; i += kSelThreads) s_keys[i - begin] = __float_as_uint(w[kept[i]]);
+  cluster.sync();  // and no CTA leaves while another reads its counts
+  if (!in_turn || cached) {
+    for (uint32_t i = begin + tid; i < end; i += kSelThreads) w_out[i] = in_turn ? __uint_as_float(s_keys[i - begin]) : __ldg(w + kept[i]);
+    for (uint32_t i = want + rank * kSelThreads + tid; i < len; i += ctas * kSelThreads) w_out[i] = 0.f;
+  }
+  if (p.dst_table) move_rows(p, b, h, kept, begin, end, s_rows);
 }
 
 constexpr int kMoveThreads = 256;
-constexpr uint32_t kMoveRows = 64;
 
-// Weights of the kept tokens to the front of weights_out, zeros behind them up to the old length;
-// weights_out may be weights: a batch of ranks is read before any of it is written.
-__device__ void move_weights(const EvictParams &p, uint32_t b, uint32_t h) {
+// Weights of the kept tokens to the front of weights_out (which is weights) and zeros behind them, for
+// rows longer than the selection's CTAs hold: a batch of ranks is read before any of it is written.
+__global__ void __launch_bounds__(kMoveThreads) move_weights_kernel(const __grid_constant__ EvictParams p) {
   constexpr uint32_t per = 8;
+  const uint32_t h = blockIdx.x, b = blockIdx.y;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const float *w = p.weights + (int64_t)b * p.w_req + (int64_t)h * p.w_head;
   float *o = p.weights_out + (int64_t)b * p.wo_req + (int64_t)h * p.wo_head;
   const int32_t *kept = p.kept + ((uint64_t)b * p.c.n_heads + h) * p.keep;
@@ -265,71 +342,13 @@ __device__ void move_weights(const EvictParams &p, uint32_t b, uint32_t h) {
   for (uint32_t i = n + threadIdx.x; i < len; i += kMoveThreads) o[i] = 0.f;
 }
 
-__device__ __forceinline__ int32_t dst_page(const EvictParams &p, uint32_t b, uint32_t i) {
-  const uint32_t vb = i / p.c.block_size;
-  if (vb >= p.dst_blocks) return -1;
-  const int32_t pg = __ldg(p.dst_table + (uint64_t)b * p.dst_blocks + vb);
-  return pg > 0 && (uint32_t)pg < p.c.num_blocks ? pg : -1;
-}
-
-// To fresh pages: kMoveRows ranks of one (request, head) per CTA; the last x block moves weights.
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int64_t s_src[2][kMoveRows], s_dst[2][kMoveRows];
-  const uint32_t h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (blockIdx.x == gridDim.x - 1) {
-    move_weights(p, b, h);
-    return;
-  }
-  const uint32_t n = (uint32_t)p.new_lens[b], base = blockIdx.x * kMoveRows;
-  if (base >= n) return;
-  const uint32_t rows = min(kMoveRows, n - base);
-  if (tid < rows) {
-    const uint32_t i = base + tid;
-    const uint32_t t = (uint32_t)p.kept[((uint64_t)b * p.c.n_heads + h) * p.keep + i];
-    const int32_t sp = page_of(p.c, b, t / p.c.block_size), dp = dst_page(p, b, i);
-    const uint32_t sr = t % p.c.block_size, dr = i % p.c.block_size;
-    s_src[0][tid] = (int64_t)sp * p.c.k_page + (int64_t)h * p.c.k_head + (int64_t)sr * p.c.k_row;
-    s_src[1][tid] = (int64_t)sp * p.c.v_page + (int64_t)h * p.c.v_head + (int64_t)sr * p.c.v_row;
-    s_dst[0][tid] = dp < 0 ? -1 : (int64_t)dp * p.c.k_page + (int64_t)h * p.c.k_head + (int64_t)dr * p.c.k_row;
-    s_dst[1][tid] = dp < 0 ? -1 : (int64_t)dp * p.c.v_page + (int64_t)h * p.c.v_head + (int64_t)dr * p.c.v_row;
-    if (dp < 0 && h == 0 && p.out_of_range) atomicAdd(p.out_of_range, 1u);
-  }
-  __syncthreads();
-  const uint32_t words = p.row_bytes / 16, side = rows * words, total = 2 * side;
-  constexpr int kUnroll = 8;
-  for (uint32_t at = tid; at < total; at += kMoveThreads * kUnroll) {
-    int4 x[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint32_t e = at + u * kMoveThreads;
-      if (e < total) {
-        const uint32_t s = e >= side, in = e - s * side, r = in / words, q = in % words;
-        x[u] = *reinterpret_cast<const int4 *>((s ? p.c.v : p.c.k) + s_src[s][r] + 16 * q);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint32_t e = at + u * kMoveThreads;
-      if (e < total) {
-        const uint32_t s = e >= side, in = e - s * side, r = in / words, q = in % words;
-        if (s_dst[s][r] >= 0) *reinterpret_cast<int4 *>((s ? p.c.v : p.c.k) + s_dst[s][r] + 16 * q) = x[u];
-      }
-    }
-  }
-}
-
 // In place: one CTA moves a 64-byte column of K (even blockIdx.x) or V of one (request, head),
-// kColumnRows ranks at a time; the last x block moves the weights.
+// kColumnRows ranks at a time.
 constexpr int kColumnUnroll = 8;
 constexpr uint32_t kColumnRows = kMoveThreads / 4 * kColumnUnroll;
 __global__ void __launch_bounds__(kMoveThreads) move_in_place_kernel(const __grid_constant__ EvictParams p) {
   const uint32_t h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (blockIdx.x == gridDim.x - 1) {
-    move_weights(p, b, h);
-    return;
-  }
   const uint32_t is_v = blockIdx.x & 1, word = (blockIdx.x >> 1) * 4 + (tid & 3);
   const bool live = word < p.row_bytes / 16;
   uint8_t *cache = (is_v ? p.c.v : p.c.k) + (int64_t)h * (is_v ? p.c.v_head : p.c.k_head) + 16 * word;
@@ -367,7 +386,9 @@ __global__ void __launch_bounds__(kMoveThreads) move_in_place_kernel(const __gri
 cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   if (p.c.batch == 0) return cudaSuccess;
   const uint64_t cap = (uint64_t)p.c.max_blocks * p.c.block_size;
-  // CTAs per row: pieces of 1024 tokens while the GPU has room for more CTAs, of 8192 otherwise
+  // CTAs per row: pieces of 1024 tokens while the GPU has room for more CTAs, of 8192 otherwise. (One
+  // row of 64-token pages per head, 16000 tokens, 8 heads: 19 us against 28 us with a CTA per row; 96
+  // rows of up to 32768 tokens: 92 us with four CTAs per row, 98 us with eight.)
   const uint64_t rows = (uint64_t)p.c.batch * p.c.n_heads;
   uint32_t ctas = 1;
   while (ctas < 8 && cap > 1024ull * ctas && (rows * ctas < 2ull * sms || cap > 8192ull * ctas)) ctas *= 2;
@@ -402,15 +423,17 @@ cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kMoveThreads);
   cfg.dynamicSmemBytes = 0;
-  const uint64_t most = cap < p.keep ? cap : p.keep;
-  if (p.dst_table) {
-    cfg.gridDim = dim3((unsigned)((most + kMoveRows - 1) / kMoveRows + 1), p.c.n_heads, p.c.batch);
-    e = cudaLaunchKernelEx(&cfg, move_kernel, p);
-  } else {
-    cfg.gridDim = dim3(2 * ((p.row_bytes + 63) / 64) + 1, p.c.n_heads, p.c.batch);
+  if (!p.dst_table) {
+    cfg.gridDim = dim3(2 * ((p.row_bytes + 63) / 64), p.c.n_heads, p.c.batch);
     e = cudaLaunchKernelEx(&cfg, move_in_place_kernel, p);
+    if (e != cudaSuccess) return e;
+    count_launch();
   }
-  if (e == cudaSuccess) count_launch();
+  if (!cached && p.weights == p.weights_out) {
+    cfg.gridDim = dim3(p.c.n_heads, p.c.batch);
+    e = cudaLaunchKernelEx(&cfg, move_weights_kernel, p);
+    if (e == cudaSuccess) count_launch();
+  }
   return e;
 }
 

@@ -269,6 +269,9 @@ int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *r, void 
         "%s: dst_page_table must cover keep (%u) slots", op, r->keep);
   CHECK(r->w_len >= cap && r->wo_len >= cap, "%s: weights must cover max_num_blocks_per_seq * block_size tokens", op);
   CHECK((uint64_t)cache->batch * cache->n_heads <= 0x7FFFFFFFull / 8, "%s: too many requests and heads", op);
+  CHECK(r->weights != r->weights_out || (r->weights_strides[0] == r->weights_out_strides[0] &&
+                                         r->weights_strides[1] == r->weights_out_strides[1]),
+        "%s: weights_out must be weights itself or not overlap it", op);
   Where w{op};
   TRY(add_cache(w, cache));
   TRY(w.add(r->seq_lens, "seq_lens"));
@@ -298,6 +301,7 @@ int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *r, void 
   p.out_of_range = r->out_of_range;
   p.page = kvs::Divisor(p.c.block_size);
   p.row_bytes = cache->head_dim * (cache->dtype == KVS_DTYPE_E4M3 ? 1 : 2);
+  p.words = kvs::Divisor(p.row_bytes / 16);
   CUDA_TRY(kvs::launch_evict(p, sms, static_cast<cudaStream_t>(stream)), op);
   return KVS_OK;
 }

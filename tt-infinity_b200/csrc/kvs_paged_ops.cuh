@@ -110,6 +110,7 @@ struct EvictParams {
   uint32_t *out_of_range;
   uint32_t row_bytes;
   Divisor page;               // block_size
+  Divisor words;              // 16-byte words of a row
 };
 cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream);
 

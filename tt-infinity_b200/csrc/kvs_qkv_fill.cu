@@ -14,7 +14,10 @@
 // the norm one reduction over the row's lanes. Norm weight, cosine and sine of a pair are four
 // coefficients that stay in registers over the warp's rows:
 //     (a, b) -> (a A + b B, a C + b D) / sqrt(mean + eps)    A = wa cos, B = -wb sin, C = wa sin, D = wb cos
-// and the next rows are loaded while these are computed.
+// and the next rows are loaded while these are computed. Blocks of one warp: warps of a token differ in
+// length (queries, keys and values), and a block holds its registers until its last warp is done (72 us
+// against 60 us with blocks of two). 8192 tokens of 64 + 2 x 8 heads of 128: 57 us, 92 % of the measured
+// copy rate.
 #include "kvs_paged_ops.cuh"
 
 #include <cuda_bf16.h>
@@ -27,10 +30,7 @@ namespace kvs {
 
 namespace {
 
-#ifndef TUNE_U
-#define TUNE_U 2
-#endif
-constexpr int kUnroll = TUNE_U;  // rows in flight per lane
+constexpr int kUnroll = 2;  // rows in flight per lane
 
 template <bool kBf>
 __device__ __forceinline__ float2 widen2(uint32_t x) {
@@ -328,12 +328,10 @@ __global__ void __launch_bounds__(32) qkv_fill_kernel(const __grid_constant__ Qk
 template <bool kBf, bool kInter, int PP, int kLanes>
 cudaError_t run(const QkvFillParams &p, cudaStream_t stream) {
   using R = Rows<kBf, kInter, PP, kLanes>;
-#ifndef TUNE_STEPS
-#define TUNE_STEPS 8
-#endif
-  // rows per warp: as many as leave enough warps
+  // Rows per warp: many share one lookup and one set of coefficients, as long as enough warps are left.
+  // 8192 tokens of 64 + 2 x 8 heads: 57 us with up to 64 rows per warp, 66 us with 16.
   const uint32_t steps = (p.q_heads + R::step - 1) / R::step;
-  uint32_t per = TUNE_STEPS;
+  uint32_t per = 8;
   while (per > 1 && (uint64_t)p.tokens * ((steps + per - 1) / per) < 148 * 16) per /= 2;
   const uint32_t q_parts = (steps + per - 1) / per, kv_parts = (p.c.n_heads + per * R::step - 1) / (per * R::step);
   const dim3 grid(p.tokens, q_parts + kv_parts);
