@@ -634,3 +634,37 @@ def test_refusals():
                         (dict(weights_out=f32(2, 2, 16)), "must cover"), (dict(seq_lens=n(1)), "must match")]:
         with pytest.raises(RuntimeError, match=msg):
             ops.evict_paged_kv(**dict(ev, **change))
+
+
+def run_all_three(s):
+    """Every operator once, with every argument given, on copies of the case's buffers."""
+    k, v, w = s["k"].clone(), s["v"].clone(), s["w"].clone()
+    count = torch.zeros(1, dtype=torch.int32, device="cuda")
+    g = gen(3)
+    q, kk, vv = (torch.randn((4, h, 64), generator=g).to(BF16).cuda() for h in (8, 2, 2))
+    ones = torch.ones(64, dtype=BF16, device="cuda")
+    cs = torch.rand((16, 64), generator=g).cuda()
+    out = torch.zeros_like(q)
+    new, _, _ = ops.qk_norm_rope_fill(q, kk, vv, cs, i32(range(5)), s["table"], i32([299, 39, 0, 776]), k, v, q_weight=ones,
+                                      k_weight=ones, eps=1e-5, positions=i32([[1, 2, 3, 4], [5, 6, 7, 99]]), axes=i32([0, 1] * 16),
+                                      interleaved=True, q_out=out, out_of_range=count)
+    assert new is out
+    att, lse = ops.paged_decode_attention(new, k, v, s["table"], s["lens"], scale=0.3, window=500, out=torch.zeros_like(q), return_lse=True, weights=w)
+    plain = ops.paged_decode_attention(new, k, v, s["table"], s["lens"])
+    kept, lens = ops.evict_paged_kv(k, v, s["table"], s["lens"], w, 100, first=1, recent=2, dst_page_table=s["dst"], out_of_range=count)
+    placed, _ = ops.evict_paged_kv(k, v, s["dst"], lens, w[..., :112].clone(), 50)
+    return [new, att, lse, plain, kept, lens, placed, w, count, k.nan_to_num(), v.nan_to_num()]
+
+
+def test_compiled_and_ctypes_calls_agree(monkeypatch):
+    from kvcache_manager import _native
+
+    s = small_case(90)
+    assert _native.load_opcall(), "the compiled entry is built beside the library"
+    with monkeypatch.context() as m:
+        m.setattr(ops, "_paged_cache", None)  # the ctypes path cannot be taken
+        fast = run_all_three(s)
+    with monkeypatch.context() as m:
+        m.setattr(_native, "opcall", False)
+        slow = run_all_three(s)
+    assert all(torch.equal(a, b) for a, b in zip(fast, slow)) and int(fast[8]) == 1

@@ -63,8 +63,46 @@ def build_fastcall(force: bool = False) -> Path:
     return out
 
 
+OPCALL_SRC = CSRC / "pyext" / "kvs_opcall.cpp"
+
+
+def opcall_path() -> Path:
+    import sysconfig
+
+    return PKG / "kvcache_manager" / ("_opcall" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_opcall(force: bool = False) -> Path:
+    """The CPython module of the operators on a paged cache (g++ against torch's headers and
+    libraries, which the package's import of torch has loaded; it calls libkvs_b200.so through
+    function pointers)."""
+    import sysconfig
+
+    import torch
+
+    out = opcall_path()
+    deps = [OPCALL_SRC, ROOT / "include" / "kvs.h", Path(torch.__file__)]
+    if not force and out.exists() and all(d.stat().st_mtime < out.stat().st_mtime for d in deps):
+        return out
+    home = Path(torch.__file__).parent
+    cuda = Path(NVCC).resolve().parents[1]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", sysconfig.get_paths()["include"], "-I", str(ROOT / "include"), "-isystem", str(home / "include"),
+           "-isystem", str(home / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda / "include"),
+           str(OPCALL_SRC), "-o", str(out) + ".tmp", "-L", str(home / "lib"), "-ltorch_python", "-ltorch_cpu",
+           "-lc10_cuda", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("g++ failed building the _opcall module")
+    os.replace(str(out) + ".tmp", out)
+    return out
+
+
 def build(debug: bool = False, verbose: bool = False, force: bool = False) -> Path:
     build_fastcall(force)
+    build_opcall(force)
     if not force and not needs_build(OUT):
         return OUT
     flags = ARCH + [

@@ -383,6 +383,29 @@ def _bind_fastcall(lib) -> None:
     fastcall = _fastcall
 
 
+opcall = None  # the CPython module of the operators on a paged cache; False: not built
+
+
+def load_opcall():
+    """The _opcall module (built beside the library by build.py, against the torch that is loaded),
+    bound to the loaded library, or False without it: ops then calls through ctypes."""
+    global opcall
+    if opcall is None:
+        lib = load()
+        try:
+            import torch  # noqa: F401 - its libraries are what the module links to
+
+            from . import _opcall
+        except ImportError:
+            opcall = False
+            return opcall
+        addr = lambda fn: C.cast(fn, C.c_void_p).value
+        _opcall.bind(addr(lib.kvs_qk_norm_rope_fill), addr(lib.kvs_decode_attention_workspace),
+                     addr(lib.kvs_paged_decode_attention), addr(lib.kvs_evict_paged))
+        opcall = _opcall
+    return opcall
+
+
 def check(rc: int) -> None:
     if rc != OK:
         msg = load().kvs_last_error().decode(errors="replace")

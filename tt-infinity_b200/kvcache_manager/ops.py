@@ -299,8 +299,8 @@ def _stream(device: Any):
 
 
 def _check_counter(t: Any) -> None:
-    if t is not None and t.dtype != _torch().int32:
-        raise RuntimeError("out_of_range must be an int32 tensor")
+    if t is not None and (t.dtype != _torch().int32 or t.numel() < 1):
+        raise RuntimeError("out_of_range must be an int32 tensor of one element")
 
 
 def _ptr(t: Any):
@@ -335,6 +335,12 @@ def qk_norm_rope_fill(q: Any, k: Any, v: Any, cos_sin: Any, cu_seqlens: Any, pag
     is outside cos_sin stores neither and gets a zero q_out row; out_of_range (int32, one element)
     counts both. Tokens behind the last sequence are left as they were in a given q_out and are zero
     in one allocated here. Two tokens must not share a slot. Asynchronous on the current stream."""
+    fast = _native.opcall if _native.opcall is not None else _native.load_opcall()
+    if fast:
+        done = fast.fill(q, k, v, cos_sin, cu_seqlens, page_table, start_positions, cache_k, cache_v, q_weight, k_weight,
+                         eps, positions, axes, interleaved, k_scale, v_scale, q_out, out_of_range)
+        if done is not NotImplemented:
+            return done, cache_k, cache_v
     torch = _torch()
     cache = _paged_cache(cache_k, cache_v, page_table, k_scale, v_scale)
     dev = cache_k.device
@@ -413,6 +419,12 @@ def paged_decode_attention(q: Any, cache_k: Any, cache_v: Any, page_table: Any, 
     evict_paged_kv chooses by: weights_out (default: weights itself) becomes weights plus each token's
     softmax weight summed over the KV head's query heads, for the tokens below seq_lens. Equal calls
     give equal bits. Asynchronous on the current stream; no backward pass."""
+    fast = _native.opcall if _native.opcall is not None else _native.load_opcall()
+    if fast:
+        done = fast.attend(q, cache_k, cache_v, page_table, seq_lens, scale, window, k_scale, v_scale, out, return_lse,
+                           weights, weights_out)
+        if done is not NotImplemented:
+            return done
     torch = _torch()
     cache = _paged_cache(cache_k, cache_v, page_table, k_scale, v_scale)
     dev = cache_k.device
@@ -480,6 +492,12 @@ def evict_paged_kv(cache_k: Any, cache_v: Any, page_table: Any, seq_lens: Any, w
     (default: weights itself) receives the kept tokens' weights, then zeros up to seq_lens. Keys keep the
     rotation of their old positions: rotate new tokens by the `positions` of qk_norm_rope_fill.
     Asynchronous on the current stream."""
+    fast = _native.opcall if _native.opcall is not None else _native.load_opcall()
+    if fast:
+        done = fast.evict(cache_k, cache_v, page_table, seq_lens, weights, keep, first, recent, dst_page_table,
+                          weights_out, out_of_range)
+        if done is not NotImplemented:
+            return done
     torch = _torch()
     cache = _paged_cache(cache_k, cache_v, page_table, 1.0, 1.0)
     dev = cache_k.device
