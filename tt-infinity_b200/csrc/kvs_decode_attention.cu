@@ -61,8 +61,8 @@ struct Shape {
 };
 #ifndef TUNE_SUB
 #define TUNE_SUB (el == 2 && dp == 64 && nt == 1 ? 2 : 1)
-#define TUNE_BYTES (el == 1 && dp * nt <= 128 || el * dp * nt == 256 && dp == 64 ? 49152 : 98304)
-#define TUNE_CTAS (el == 1 && dp * nt <= 128 || el * dp * nt == 256 && dp == 64 ? 4 : 2)
+#define TUNE_BYTES (el == 1 && dp * nt <= 128 && nt == 1 ? 49152 : dp == 64 && nt == 2 ? 65536 : 98304)
+#define TUNE_CTAS (el == 1 && dp * nt <= 128 && nt == 1 ? 4 : dp == 64 && nt == 2 ? 3 : 2)
 #endif
 __host__ __device__ constexpr Shape shape_of(int el, int dp, int nt) {
   Shape s{};
@@ -100,9 +100,9 @@ struct Join {
 };
 
 struct Plan {  // workspace layout
-  uint64_t joins, part_o, part_ml, lse2, logits, bytes;
+  uint64_t joins, part_o, part_ml, lse2, parts, logits, bytes;
   uint32_t grid, head_tiles, tile_heads, unit_tiles, least_units;
-  bool joins_needed;
+  bool joins_needed, narrow;
 };
 
 __host__ __device__ inline uint32_t head_tiles_of(uint32_t group) { return (group + 15) / 16; }
@@ -126,6 +126,7 @@ Plan plan_of(const PagedCache &c, uint32_t q_heads, bool weights, int sms) {
   const uint64_t full = (uint64_t)sms * per_sm;
   p.grid = (uint32_t)(most < full ? most : full);
   p.joins_needed = units > 1 && p.grid > 1;
+  p.narrow = c.batch <= kThreads && (uint64_t)c.batch * c.n_heads * p.head_tiles * units < 1ull << 31;
   uint64_t off = 0;
   auto take = [&](uint64_t n) {
     const uint64_t o = off;
@@ -136,6 +137,7 @@ Plan plan_of(const PagedCache &c, uint32_t q_heads, bool weights, int sms) {
   p.part_o = take(2ull * p.grid * p.tile_heads * dp * 4);
   p.part_ml = take(2ull * p.grid * p.tile_heads * 8);
   p.lse2 = take(weights ? 4ull * c.batch * q_heads : 0);
+  p.parts = take(8ull * c.batch * c.n_heads * p.head_tiles);
   p.logits = take(weights ? 4ull * c.batch * q_heads * cap : 0);
   p.bytes = off;
   return p;
@@ -146,9 +148,11 @@ struct KernelParams {
   Join *joins;
   float *part_o;
   float2 *part_ml;
-  float *lse2;    // base-2 log-sum-exp per row, kept for the weights
+  float *lse2;    // base-2 log-sum-exp of the rows that were not split, kept for the weights
   float *logits;  // [batch][n_heads][cap][group] scores in base 2, or nullptr
-  uint32_t cap, head_tiles, group, unit_tiles, least_units;
+  uint2 *parts;   // [batch][head tiles]: first CTA and how many more hold a part
+  uint32_t cap, head_tiles, group, unit_tiles, least_units, join_blocks, pieces, join_parts;
+  bool narrow;   // at most kThreads requests, and all counts of units fit 32 bits
   Divisor page;  // block_size
 };
 
@@ -234,8 +238,9 @@ __device__ __forceinline__ Span span_of(const KernelParams &p, uint32_t b) {
   return s;
 }
 
+__device__ __forceinline__ float log2_sum(float m, float l) { return l == 0.f ? -INFINITY : m + __log2f(l); }
 __device__ __forceinline__ void store_lse(const KernelParams &p, uint64_t row, float m, float l) {
-  const float lse2 = l == 0.f ? -INFINITY : m + __log2f(l);
+  const float lse2 = log2_sum(m, l);
   if (p.a.lse) p.a.lse[row] = lse2 * kLn2;
   if (p.lse2) p.lse2[row] = lse2;
 }
@@ -273,8 +278,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
   constexpr int kSteps = DP / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *const smem = smem_raw + (-smem_addr(smem_raw) & 511);
-  __shared__ uint64_t s_scan[kWarps + 1];
-  __shared__ uint32_t s_where[2];
+  __shared__ uint64_t s_scan[kWarps];
+  __shared__ Cursor s_at;
   __shared__ uint32_t s_mask[kWarps][C::stages][C::sub];
   __shared__ float s_m[C::heads], s_l[C::heads];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -283,53 +288,79 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
 
   // ---- this CTA's run of units
   const uint32_t hh_n = c.n_heads * p.head_tiles;
-  uint64_t total = 0, mine = 0;
-  for (uint32_t base = 0; base < c.batch; base += kThreads) {
-    mine = base + tid < c.batch ? span_of(p, base + tid).units : 0;
-    uint64_t x = mine;
-    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
-    total += x;
-  }
-  if (lane == 0) s_scan[warp] = total;
-  __syncthreads();
-  total = 0;
-  for (int w = 0; w < kWarps; ++w) total += s_scan[w];
-  total *= hh_n;
-  const uint64_t quota = max((uint64_t)p.least_units, (total + gridDim.x - 1) / gridDim.x);
-  const uint64_t begin = quota * blockIdx.x;
   if (tid == 0) p.joins[blockIdx.x].followers = 0;
-  if (begin >= total) return;
-  // request that holds unit `begin`: the requests' units times hh_n, scanned kThreads at a time
-  uint64_t run = 0;
-  for (uint32_t base = 0; base < c.batch; base += kThreads) {
-    const uint64_t val = c.batch <= kThreads ? mine : (base + tid < c.batch ? span_of(p, base + tid).units : 0);
-    uint64_t incl = val;
+  uint64_t quota;
+  // The loads run ahead of the products, across the ends of runs: `ahead` is where the loads are.
+  Cursor at;
+  if (p.narrow) {  // one request per thread and 32-bit counts: one scan
+    Span mine{};
+    if (tid < c.batch) mine = span_of(p, tid);
+    uint32_t incl = mine.units;
     for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t y = __shfl_up_sync(~0u, incl, o);
+      const uint32_t y = __shfl_up_sync(~0u, incl, o);
       if (lane >= o) incl += y;
     }
-    __syncthreads();
     if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
-    uint64_t before = run, all = 0;
+    uint32_t total = 0;
     for (int w = 0; w < kWarps; ++w) {
-      if (w < (int)warp) before += s_scan[w];
-      all += s_scan[w];
+      if (w < (int)warp) incl += (uint32_t)s_scan[w];
+      total += (uint32_t)s_scan[w];
     }
-    const uint64_t lo = (before + incl - val) * hh_n, hi = (before + incl) * hh_n;
-    if (val && lo <= begin && begin < hi) {
-      const uint64_t in = begin - lo;
-      s_where[0] = base + tid;
-      s_where[1] = (uint32_t)(in / val);       // head tile
-      s_scan[kWarps] = in % val;               // unit within it
+    total *= hh_n;
+    const uint32_t share = max(p.least_units, (total + gridDim.x - 1) / gridDim.x), begin = share * blockIdx.x;
+    if (begin >= total) return;
+    const uint32_t lo = (incl - mine.units) * hh_n;
+    if (mine.units && lo <= begin && begin < incl * hh_n) {
+      const uint32_t in = begin - lo, hh = in / mine.units;
+      s_at = Cursor{tid, hh, in - hh * mine.units, min(share, total - begin), mine};
     }
-    run += all;
     __syncthreads();
-    if (run * hh_n > begin) break;
+    at = s_at;
+    quota = share;
+  } else {
+    uint64_t total = 0;
+    for (uint32_t base = 0; base < c.batch; base += kThreads) {
+      uint64_t x = base + tid < c.batch ? span_of(p, base + tid).units : 0;
+      for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+      total += x;
+    }
+    if (lane == 0) s_scan[warp] = total;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < kWarps; ++w) total += s_scan[w];
+    total *= hh_n;
+    quota = max((uint64_t)p.least_units, (total + gridDim.x - 1) / gridDim.x);
+    const uint64_t begin = quota * blockIdx.x;
+    if (begin >= total) return;
+    // request that holds unit `begin`: the requests' units times hh_n, scanned kThreads at a time
+    uint64_t run = 0;
+    for (uint32_t base = 0; base < c.batch; base += kThreads) {
+      const uint64_t val = base + tid < c.batch ? span_of(p, base + tid).units : 0;
+      uint64_t incl = val;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(~0u, incl, o);
+        if (lane >= o) incl += y;
+      }
+      __syncthreads();
+      if (lane == 31) s_scan[warp] = incl;
+      __syncthreads();
+      uint64_t before = run, all = 0;
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < (int)warp) before += s_scan[w];
+        all += s_scan[w];
+      }
+      const uint64_t lo = (before + incl - val) * hh_n, hi = (before + incl) * hh_n;
+      if (val && lo <= begin && begin < hi) {
+        const uint64_t in = begin - lo;
+        s_at = Cursor{base + tid, (uint32_t)(in / val), (uint32_t)(in % val), min(quota, total - begin), span_of(p, base + tid)};
+      }
+      run += all;
+      __syncthreads();
+      if (run * hh_n > begin) break;
+    }
+    at = s_at;
   }
-  // The loads run ahead of the products, across the ends of runs: `ahead` is where the loads are.
-  Cursor at{s_where[0], s_where[1], (uint32_t)s_scan[kWarps], min(quota, total - begin), {}};
-  at.span = span_of(p, at.b);
   Cursor ahead = at;
 
   const uint32_t ring = smem_addr(smem) + warp * C::stages * C::stage;
@@ -346,6 +377,26 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
   auto swizzle = [](uint32_t row) constexpr -> uint32_t { return C::pitch >= 128 ? (row & 7) : ((row >> 1) & 3); };
   const uint32_t my_place = my_row * C::pitch + ((my_chunk ^ swizzle(my_row)) << 4);
 
+  uint32_t bq[kSteps][NT][2];
+  // Queries of a run, as they are in memory. The product's index 2j + {0, 1} of a step is element
+  // 2j + {0, 1} (and 2j + 8 + {0, 1} eight further on); for an e4m3 cache 4j + {0, 1} (4j + 2 + {0, 1}),
+  // the order in which four bytes of a key row come out of a matrix load.
+  auto load_queries = [&](const Cursor &of) {
+    const uint32_t first_head = of.hh / p.head_tiles * p.group, g_first = of.hh % p.head_tiles * C::heads;
+    const uint32_t j = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint32_t g = g_first + nt * 8 + (lane >> 2);
+      const uint32_t *qr = reinterpret_cast<const uint32_t *>(p.a.q + (int64_t)of.b * p.a.q_req + (int64_t)(first_head + g) * p.a.q_head);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t d = k8 ? 16 * s + 4 * j + 2 * half : 16 * s + 8 * half + 2 * j;
+          bq[s][nt][half] = g < p.group && d < c.head_dim ? __ldg(qr + d / 2) : 0u;
+        }
+    }
+  };
   // ---- loads
   constexpr uint32_t stride = kWarps * C::sub;  // tiles between a warp's steps
   uint32_t load_tile_at = ahead.begin(p) + warp * C::sub, load_end = ahead.end(p);
@@ -446,32 +497,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
   settle();
 #pragma unroll
   for (int s = 0; s < C::stages - 1; ++s) issue(s);
+  load_queries(at);
   uint32_t stage = 0;
   const uint32_t k_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_row = (lane & 7) + (lane >> 4) * 8;
   const uint32_t k_place = k_row * C::pitch + (((lane >> 4) ^ swizzle(k_row)) << 4);
   const uint32_t v_place = v_row * C::pitch + ((((lane >> 3) & 1) ^ swizzle(v_row)) << 4);
-
-  uint32_t bq[kSteps][NT][2];
-  // Queries of a run, as they are in memory. The product's index 2j + {0, 1} of a step is element
-  // 2j + {0, 1} (and 2j + 8 + {0, 1} eight further on); for an e4m3 cache 4j + {0, 1} (4j + 2 + {0, 1}),
-  // the order in which four bytes of a key row come out of a matrix load.
-  auto load_queries = [&](const Cursor &of) {
-    const uint32_t first_head = of.hh / p.head_tiles * p.group, g_first = of.hh % p.head_tiles * C::heads;
-    const uint32_t j = lane & 3;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const uint32_t g = g_first + nt * 8 + (lane >> 2);
-      const uint32_t *qr = reinterpret_cast<const uint32_t *>(p.a.q + (int64_t)of.b * p.a.q_req + (int64_t)(first_head + g) * p.a.q_head);
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t d = k8 ? 16 * s + 4 * j + 2 * half : 16 * s + 8 * half + 2 * j;
-          bq[s][nt][half] = g < p.group && d < c.head_dim ? __ldg(qr + d / 2) : 0u;
-        }
-    }
-  };
-  load_queries(at);
 
   while (at.left) {
     const uint32_t b = at.b, h = at.hh / p.head_tiles, g0 = (at.hh % p.head_tiles) * C::heads;
@@ -780,58 +810,71 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
           }
         }
         // units of this (request, head tile) after the ones taken here, over runs of `quota`
-        if (lane == 0 && starts)
-          p.joins[blockIdx.x] = Join{b, at.hh, (uint32_t)((at.span.units - at.take() + quota - 1) / quota), 0};
+        if (lane == 0 && starts) {
+          const uint32_t followers = (uint32_t)((at.span.units - at.take() + quota - 1) / quota);
+          p.joins[blockIdx.x] = Join{b, at.hh, followers, 0};
+          p.parts[(uint64_t)b * hh_n + at.hh] = make_uint2(blockIdx.x, followers);
+        }
       }
+      if (lane == 0 && starts && ends) p.parts[(uint64_t)b * hh_n + at.hh] = make_uint2(blockIdx.x, 0);
     }
     at = following;
   }
 }
 
-// Joins the partials of the (request, head tile) whose first units CTA blockIdx.x took: slot 1 of
-// that CTA, then slot 0 of the CTAs after it, in that order. One block per 16 elements of 8 heads (one
-// fragment), its eight warps taking every eighth partial.
+// Joins the partials of a (request, head tile): slot 1 of the CTA that took its first units, then slot 0
+// of the CTAs after it. Blocks stand for CTAs or, where there are fewer, for (request, head tile)s. A piece is 16 elements of 8 heads (one fragment); a block takes
+// p.pieces of them, each by 8 / p.pieces warps that take every so many partials and add up in order.
 template <int DP, int NT, bool k8>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ KernelParams p) {
+__device__ __forceinline__ void join_part(const KernelParams &p, uint32_t block) {
   constexpr int kSteps = DP / 16;
   constexpr uint32_t tile_heads = 8 * NT;
   __shared__ float4 s_sum[8][32];
-  __shared__ float s_red[8][8];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Join j = p.joins[blockIdx.x];
+  __shared__ float s_l[8][8];
+  __shared__ float s_top[8][8];
+  const uint32_t groups = NT * kSteps / p.pieces, index = block / groups;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t piece = block % groups * p.pieces + warp % p.pieces, sub = warp / p.pieces, subs = 8 / p.pieces;
+  Join j;
+  uint32_t cta = index;
+  if (p.join_parts) {
+    const uint32_t hh_n = p.a.c.n_heads * p.head_tiles;
+    const uint2 part = p.parts[index];
+    cta = part.x;
+    j = Join{index / hh_n, index % hh_n, part.y, 0};
+  } else {
+    j = p.joins[cta];
+  }
   if (j.followers == 0) return;
-  const uint32_t nt = blockIdx.y / kSteps, s = blockIdx.y % kSteps;
+  const uint32_t nt = piece / kSteps, s = piece % kSteps;
   const uint32_t g0 = (j.hh % p.head_tiles) * tile_heads + nt * 8, h = j.hh / p.head_tiles;
-  if (g0 >= p.group || 16 * s >= p.a.c.head_dim) return;
-  const uint32_t n = j.followers + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto slot = [&](uint32_t i) -> uint64_t { return i == 0 ? 2ull * blockIdx.x + 1 : 2ull * (blockIdx.x + i); };
+  const uint32_t n = j.followers + 1;
+  auto slot = [&](uint32_t i) -> uint64_t { return i == 0 ? 2ull * cta + 1 : 2ull * (cta + i); };
   // the first partials of each warp are on their way while the maxima are found
   auto sums_of = [&](uint32_t i) {
     return reinterpret_cast<const float4 *>(p.part_o)[(slot(i) * NT * kSteps + nt * kSteps + s) * 32 + lane];
   };
   auto stats_of = [&](uint32_t i) { return *reinterpret_cast<const float4 *>(p.part_ml + slot(i) * tile_heads + nt * 8 + 2 * (lane & 3)); };
-  constexpr int kEarly = 5;
+  constexpr int kEarly = 4;
   float4 y[kEarly], ml[kEarly];
 #pragma unroll
   for (int e = 0; e < kEarly; ++e)
-    if (warp + 8 * e < n) {
-      y[e] = sums_of(warp + 8 * e);
-      ml[e] = stats_of(warp + 8 * e);
+    if (sub + subs * e < n) {
+      y[e] = sums_of(sub + subs * e);
+      ml[e] = stats_of(sub + subs * e);
     }
   // maximum of each of the eight heads: lane % 8 is the head
   float M = -INFINITY;
-  for (uint32_t i = warp * 4 + lane / 8; i < n; i += 32) M = fmaxf(M, p.part_ml[slot(i) * tile_heads + nt * 8 + lane % 8].x);
+#pragma unroll 2
+  for (uint32_t i = sub * 4 + lane / 8; i < n; i += 4 * subs) M = fmaxf(M, p.part_ml[slot(i) * tile_heads + nt * 8 + lane % 8].x);
   M = fmaxf(M, __shfl_xor_sync(~0u, M, 8));
   M = fmaxf(M, __shfl_xor_sync(~0u, M, 16));
-  if (lane < 8) s_red[warp][lane] = M;
-  __syncthreads();
-  float top[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    top[i] = -INFINITY;
-    for (int w = 0; w < 8; ++w) top[i] = fmaxf(top[i], s_red[w][2 * (lane & 3) + i]);
+  if (subs > 1) {
+    if (lane < 8) s_top[warp][lane] = M;
+    __syncthreads();
+    for (uint32_t w = warp % p.pieces; w < 8; w += p.pieces) M = fmaxf(M, s_top[w][lane % 8]);
   }
-  __syncthreads();
+  const float top[2] = {__shfl_sync(~0u, M, 2 * (lane & 3)), __shfl_sync(~0u, M, 2 * (lane & 3) + 1)};
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   float L[2] = {0.f, 0.f};
   auto add = [&](const float4 &o, const float4 &st) {
@@ -845,25 +888,26 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Kerne
   };
 #pragma unroll
   for (int e = 0; e < kEarly; ++e)
-    if (warp + 8 * e < n) add(y[e], ml[e]);
+    if (sub + subs * e < n) add(y[e], ml[e]);
 #pragma unroll 4
-  for (uint32_t i = warp + 8 * kEarly; i < n; i += 8) add(sums_of(i), stats_of(i));
-  s_sum[warp][lane] = x;
-  if (lane < 4) {
-    s_red[warp][2 * lane] = L[0];
-    s_red[warp][2 * lane + 1] = L[1];
-  }
-  __syncthreads();
-  if (warp) return;
-#pragma unroll
-  for (int w = 1; w < 8; ++w) {
-    const float4 y = s_sum[w][lane];
-    x.x += y.x;
-    x.y += y.y;
-    x.z += y.z;
-    x.w += y.w;
-    L[0] += s_red[w][2 * (lane & 3)];
-    L[1] += s_red[w][2 * (lane & 3) + 1];
+  for (uint32_t i = sub + subs * kEarly; i < n; i += subs) add(sums_of(i), stats_of(i));
+  if (subs > 1) {
+    s_sum[warp][lane] = x;
+    if (lane < 4) {
+      s_l[warp][2 * lane] = L[0];
+      s_l[warp][2 * lane + 1] = L[1];
+    }
+    __syncthreads();
+    if (sub) return;
+    for (uint32_t w = warp + p.pieces; w < 8; w += p.pieces) {
+      const float4 z = s_sum[w][lane];
+      x.x += z.x;
+      x.y += z.y;
+      x.z += z.z;
+      x.w += z.w;
+      L[0] += s_l[w][2 * (lane & 3)];
+      L[1] += s_l[w][2 * (lane & 3) + 1];
+    }
   }
   const uint32_t r = lane >> 2;
 #pragma unroll
@@ -880,33 +924,84 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Kerne
   }
 }
 
-// weights_out[b, h, t] = weights[b, h, t] + sum over the heads of the group of 2^(score - lse).
-__global__ void __launch_bounds__(256) add_weights_kernel(const __grid_constant__ KernelParams p) {
+// weights_out[b, h, t] = weights[b, h, t] + sum over the heads of the group of 2^(score - lse), for
+// kWeightTokens tokens. The log-sum-exp of a head that was split is found from its parts here, a warp per head, so
+// that this needs no wait for the join.
+constexpr uint32_t kWeightTokens = 1024;
+template <int NT>
+__device__ __forceinline__ void add_weights(const KernelParams &p, uint32_t block) {
   extern __shared__ float s_lse[];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const uint32_t h = blockIdx.y, b = blockIdx.z;
+  constexpr uint32_t tile_heads = 8 * NT;
+  const uint32_t chunks = (p.cap + kWeightTokens - 1) / kWeightTokens, chunk = block % chunks, row = block / chunks;
+  const uint32_t h = row % p.a.c.n_heads, b = row / p.a.c.n_heads, lane = threadIdx.x & 31;
   const Span span = span_of(p, b);
-  const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-  if (blockIdx.x * 256 >= min(span.len, p.a.w_len)) return;
-  for (uint32_t g = threadIdx.x; g < p.group; g += 256) s_lse[g] = p.lse2[(uint64_t)b * p.a.q_heads + h * p.group + g];
-  __syncthreads();
-  if (t >= min(span.len, p.a.w_len)) return;
-  float x = 0.f;
-  if (t >= span.low) {
-    const float *lg = p.logits + (((uint64_t)b * p.a.c.n_heads + h) * p.cap + t) * p.group;
-    auto weight = [&](float score, uint32_t g) { return s_lse[g] == -INFINITY ? 0.f : exp2_fast(score - s_lse[g]); };
-    if (p.group % 4 == 0) {
-#pragma unroll 2
-      for (uint32_t g = 0; g < p.group; g += 4) {
-        const float4 y = *reinterpret_cast<const float4 *>(lg + g);
-        x += (weight(y.x, g) + weight(y.y, g + 1)) + (weight(y.z, g + 2) + weight(y.w, g + 3));
-      }
+  if (chunk * kWeightTokens >= span.len) return;
+  for (uint32_t g = threadIdx.x >> 5; g < p.group; g += 8) {
+    const uint32_t hh = h * p.head_tiles + g / tile_heads;
+    const uint2 part = p.parts[(uint64_t)b * (p.a.c.n_heads * p.head_tiles) + hh];
+    float lse2;
+    if (part.y == 0) {
+      lse2 = p.lse2[(uint64_t)b * p.a.q_heads + h * p.group + g];
     } else {
-      for (uint32_t g = 0; g < p.group; ++g) x += weight(lg[g], g);
+      auto stats = [&](uint32_t i) { return p.part_ml[(i == 0 ? 2ull * part.x + 1 : 2ull * (part.x + i)) * tile_heads + g % tile_heads]; };
+      float M = -INFINITY, L = 0.f;
+      for (uint32_t i = lane; i <= part.y; i += 32) M = fmaxf(M, stats(i).x);
+      for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+      for (uint32_t i = lane; i <= part.y; i += 32) {
+        const float2 ml = stats(i);
+        L += rebase(ml.x, ml.y, M) * ml.y;
+      }
+      for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
+      lse2 = log2_sum(M, L);
     }
+    if (lane == 0) s_lse[g] = lse2;
   }
-  p.a.weights_out[(int64_t)b * p.a.wo_req + (int64_t)h * p.a.wo_head + t] =
-      p.a.weights[(int64_t)b * p.a.w_req + (int64_t)h * p.a.w_head + t] + x;
+  __syncthreads();
+  const uint32_t end = min(span.len, p.a.w_len);
+  const float *w = p.a.weights + (int64_t)b * p.a.w_req + (int64_t)h * p.a.w_head;
+  float *w_out = p.a.weights_out + (int64_t)b * p.a.wo_req + (int64_t)h * p.a.wo_head;
+  const float *rows = p.logits + ((uint64_t)b * p.a.c.n_heads + h) * p.cap * p.group;
+  auto weight = [&](float score, uint32_t g) { return s_lse[g] == -INFINITY ? 0.f : exp2_fast(score - s_lse[g]); };
+  constexpr uint32_t per = kWeightTokens / 256;
+  float x[per];
+#pragma unroll
+  for (uint32_t i = 0; i < per; ++i) {
+    const uint32_t t = chunk * kWeightTokens + i * 256 + threadIdx.x;
+    x[i] = t < end ? w[t] : 0.f;
+  }
+  if (p.group % 4 == 0) {
+    for (uint32_t g = 0; g < p.group; g += 4) {
+      float4 y[per];
+#pragma unroll
+      for (uint32_t i = 0; i < per; ++i) {
+        const uint32_t t = chunk * kWeightTokens + i * 256 + threadIdx.x;
+        y[i] = t >= span.low && t < end ? *reinterpret_cast<const float4 *>(rows + (uint64_t)t * p.group + g)
+                                        : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < per; ++i) x[i] += (weight(y[i].x, g) + weight(y[i].y, g + 1)) + (weight(y[i].z, g + 2) + weight(y[i].w, g + 3));
+    }
+  } else {
+    for (uint32_t g = 0; g < p.group; ++g)
+#pragma unroll
+      for (uint32_t i = 0; i < per; ++i) {
+        const uint32_t t = chunk * kWeightTokens + i * 256 + threadIdx.x;
+        if (t >= span.low && t < end) x[i] += weight(rows[(uint64_t)t * p.group + g], g);
+      }
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < per; ++i) {
+    const uint32_t t = chunk * kWeightTokens + i * 256 + threadIdx.x;
+    if (t < end) w_out[t] = x[i];
+  }
+}
+
+// What is left to do after all units: the first join_blocks blocks join, the others add up weights.
+template <int DP, int NT, bool k8>
+__global__ void __launch_bounds__(256, 3) finish_kernel(const __grid_constant__ KernelParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (blockIdx.x < p.join_blocks) join_part<DP, NT, k8>(p, blockIdx.x);
+  else add_weights<NT>(p, blockIdx.x - p.join_blocks);
 }
 
 template <class K, class... Args>
@@ -944,14 +1039,20 @@ cudaError_t run(const KernelParams &kp, const Plan &plan, cudaStream_t stream) {
   count_launch();
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (plan.joins_needed) {
-    e = launch_after(join_kernel<DP, NT, kKind == kKindE4m3>, dim3(plan.grid, NT * (DP / 16)), dim3(256), 0, stream, kp);
-    if (e != cudaSuccess) return e;
-  }
-  if (kp.logits) {
-    const dim3 grid((kp.cap + 255) / 256, kp.a.c.n_heads, kp.a.c.batch);
-    e = launch_after(add_weights_kernel, grid, dim3(256), 4ull * kp.group, stream, kp);
-  }
+  KernelParams fp = kp;
+  // Fragments a joining block takes: up to eight, a warp each, which suits requests of a few parts; where
+  // a (request, head) may have many, fewer, with more warps for each.
+  const uint64_t tiles = (uint64_t)kp.a.c.batch * kp.a.c.n_heads * kp.head_tiles;
+  const uint32_t pieces = NT * (DP / 16), spread = (uint32_t)(plan.grid / tiles);
+  fp.pieces = spread >= 16 ? 1 : (spread >= 8 ? 2 : (spread >= 4 ? 4 : 8));
+  if (fp.pieces > pieces) fp.pieces = pieces;
+  fp.join_parts = tiles < plan.grid;
+  fp.join_blocks = plan.joins_needed ? (uint32_t)(fp.join_parts ? tiles : plan.grid) * (pieces / fp.pieces) : 0;
+  uint64_t blocks = fp.join_blocks;
+  if (kp.logits) blocks += (uint64_t)((kp.cap + kWeightTokens - 1) / kWeightTokens) * kp.a.c.n_heads * kp.a.c.batch;
+  if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+  if (blocks)
+    e = launch_after(finish_kernel<DP, NT, kKind == kKindE4m3>, dim3((unsigned)blocks), dim3(256), kp.logits ? 4ull * kp.group : 0, stream, fp);
   return e;
 }
 
@@ -982,11 +1083,13 @@ cudaError_t launch_decode_attention(const DecodeAttentionParams &a, int sms, cud
   kp.joins = reinterpret_cast<Join *>(a.workspace + plan.joins);
   kp.part_o = reinterpret_cast<float *>(a.workspace + plan.part_o);
   kp.part_ml = reinterpret_cast<float2 *>(a.workspace + plan.part_ml);
+  kp.parts = reinterpret_cast<uint2 *>(a.workspace + plan.parts);
   kp.cap = a.c.max_blocks * a.c.block_size;
   kp.head_tiles = plan.head_tiles;
   kp.unit_tiles = plan.unit_tiles;
   kp.page = Divisor(a.c.block_size);
   kp.least_units = plan.least_units;
+  kp.narrow = plan.narrow;
   kp.group = a.q_heads / a.c.n_heads;
   if (a.weights_out) {
     kp.lse2 = reinterpret_cast<float *>(a.workspace + plan.lse2);
