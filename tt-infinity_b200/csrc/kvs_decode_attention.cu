@@ -151,7 +151,7 @@ struct KernelParams {
   float *lse2;    // base-2 log-sum-exp of the rows that were not split, kept for the weights
   float *logits;  // [batch][n_heads][cap][group] scores in base 2, or nullptr
   uint2 *parts;   // [batch][head tiles]: first CTA and how many more hold a part
-  uint32_t cap, head_tiles, group, unit_tiles, least_units, join_blocks, pieces, join_parts;
+  uint32_t cap, head_tiles, group, unit_tiles, least_units, join_blocks, pieces, join_parts, weight_chunk;
   bool narrow;   // at most kThreads requests, and all counts of units fit 32 bits
   Divisor page;  // block_size
 };
@@ -925,17 +925,49 @@ __device__ __forceinline__ void join_part(const KernelParams &p, uint32_t block)
 }
 
 // weights_out[b, h, t] = weights[b, h, t] + sum over the heads of the group of 2^(score - lse), for
-// kWeightTokens tokens. The log-sum-exp of a head that was split is found from its parts here, a warp per head, so
+// p.weight_chunk tokens. The log-sum-exp of a head that was split is found from its parts here, a warp per head, so
 // that this needs no wait for the join.
-constexpr uint32_t kWeightTokens = 1024;
+constexpr uint32_t kWeightTokens = 1024;  // tokens a block looks at at once
 template <int NT>
 __device__ __forceinline__ void add_weights(const KernelParams &p, uint32_t block) {
   extern __shared__ float s_lse[];
   constexpr uint32_t tile_heads = 8 * NT;
-  const uint32_t chunks = (p.cap + kWeightTokens - 1) / kWeightTokens, chunk = block % chunks, row = block / chunks;
+  const uint32_t chunks = (p.cap + p.weight_chunk - 1) / p.weight_chunk, chunk = block % chunks, row = block / chunks;
   const uint32_t h = row % p.a.c.n_heads, b = row / p.a.c.n_heads, lane = threadIdx.x & 31;
   const Span span = span_of(p, b);
-  if (chunk * kWeightTokens >= span.len) return;
+  const uint32_t begin = chunk * p.weight_chunk, end = min(min(span.len, p.a.w_len), begin + p.weight_chunk);
+  if (begin >= end) return;
+  const float *w = p.a.weights + (int64_t)b * p.a.w_req + (int64_t)h * p.a.w_head;
+  float *w_out = p.a.weights_out + (int64_t)b * p.a.wo_req + (int64_t)h * p.a.wo_head;
+  const float *rows = p.logits + ((uint64_t)b * p.a.c.n_heads + h) * p.cap * p.group;
+  constexpr uint32_t per = kWeightTokens / 256;
+  const bool fours = p.group % 4 == 0;
+  // weights and the scores of four heads of this thread's tokens t0, t0 + 256, ...
+  auto load_sums = [&](uint32_t t0, float (&x)[per]) {
+#pragma unroll
+    for (uint32_t i = 0; i < per; ++i) x[i] = t0 + i * 256 < end ? w[t0 + i * 256] : 0.f;
+  };
+  auto load_scores = [&](uint32_t t0, uint32_t g, float4 (&y)[per]) {
+#pragma unroll
+    for (uint32_t i = 0; i < per; ++i) {
+      const uint32_t t = t0 + i * 256;
+      const bool in = t >= span.low && t < end;
+      const float *at = rows + (uint64_t)t * p.group + g;
+      y[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (in && fours) {
+        y[i] = *reinterpret_cast<const float4 *>(at);
+      } else if (in) {
+        y[i].x = at[0];
+        if (g + 1 < p.group) y[i].y = at[1];
+        if (g + 2 < p.group) y[i].z = at[2];
+        if (g + 3 < p.group) y[i].w = at[3];
+      }
+    }
+  };
+  float x[per];
+  float4 y[per];
+  load_sums(begin + threadIdx.x, x);  // on their way while the log-sum-exps are found
+  load_scores(begin + threadIdx.x, 0, y);
   for (uint32_t g = threadIdx.x >> 5; g < p.group; g += 8) {
     const uint32_t hh = h * p.head_tiles + g / tile_heads;
     const uint2 part = p.parts[(uint64_t)b * (p.a.c.n_heads * p.head_tiles) + hh];
@@ -954,45 +986,28 @@ __device__ __forceinline__ void add_weights(const KernelParams &p, uint32_t bloc
       for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
       lse2 = log2_sum(M, L);
     }
-    if (lane == 0) s_lse[g] = lse2;
+    // a head without a token or a score adds nothing: exp2(-infinity - 0)
+    if (lane == 0) s_lse[g] = lse2 == -INFINITY ? 0.f : lse2;
   }
+  for (uint32_t g = p.group + threadIdx.x; g < (p.group + 3) / 4 * 4; g += 256) s_lse[g] = 0.f;
   __syncthreads();
-  const uint32_t end = min(span.len, p.a.w_len);
-  const float *w = p.a.weights + (int64_t)b * p.a.w_req + (int64_t)h * p.a.w_head;
-  float *w_out = p.a.weights_out + (int64_t)b * p.a.wo_req + (int64_t)h * p.a.wo_head;
-  const float *rows = p.logits + ((uint64_t)b * p.a.c.n_heads + h) * p.cap * p.group;
-  auto weight = [&](float score, uint32_t g) { return s_lse[g] == -INFINITY ? 0.f : exp2_fast(score - s_lse[g]); };
-  constexpr uint32_t per = kWeightTokens / 256;
-  float x[per];
-#pragma unroll
-  for (uint32_t i = 0; i < per; ++i) {
-    const uint32_t t = chunk * kWeightTokens + i * 256 + threadIdx.x;
-    x[i] = t < end ? w[t] : 0.f;
-  }
-  if (p.group % 4 == 0) {
-    for (uint32_t g = 0; g < p.group; g += 4) {
-      float4 y[per];
-#pragma unroll
-      for (uint32_t i = 0; i < per; ++i) {
-        const uint32_t t = chunk * kWeightTokens + i * 256 + threadIdx.x;
-        y[i] = t >= span.low && t < end ? *reinterpret_cast<const float4 *>(rows + (uint64_t)t * p.group + g)
-                                        : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      }
-#pragma unroll
-      for (uint32_t i = 0; i < per; ++i) x[i] += (weight(y[i].x, g) + weight(y[i].y, g + 1)) + (weight(y[i].z, g + 2) + weight(y[i].w, g + 3));
+  for (uint32_t t0 = begin + threadIdx.x; t0 < end; t0 += kWeightTokens) {
+    if (t0 >= begin + kWeightTokens) {
+      load_sums(t0, x);
+      load_scores(t0, 0, y);
     }
-  } else {
-    for (uint32_t g = 0; g < p.group; ++g)
+    for (uint32_t g = 0; g < p.group; g += 4) {
+      float4 next[per];
+      if (g + 4 < p.group) load_scores(t0, g + 4, next);
 #pragma unroll
       for (uint32_t i = 0; i < per; ++i) {
-        const uint32_t t = chunk * kWeightTokens + i * 256 + threadIdx.x;
-        if (t >= span.low && t < end) x[i] += weight(rows[(uint64_t)t * p.group + g], g);
+        x[i] += (exp2_fast(y[i].x - s_lse[g]) + exp2_fast(y[i].y - s_lse[g + 1])) + (exp2_fast(y[i].z - s_lse[g + 2]) + exp2_fast(y[i].w - s_lse[g + 3]));
+        y[i] = next[i];
       }
-  }
+    }
 #pragma unroll
-  for (uint32_t i = 0; i < per; ++i) {
-    const uint32_t t = chunk * kWeightTokens + i * 256 + threadIdx.x;
-    if (t < end) w_out[t] = x[i];
+    for (uint32_t i = 0; i < per; ++i)
+      if (t0 + i * 256 < end) w_out[t0 + i * 256] = x[i];
   }
 }
 
@@ -1022,7 +1037,7 @@ cudaError_t launch_after(K kernel, dim3 grid, dim3 block, size_t smem, cudaStrea
 }
 
 template <int kKind, int DP, int NT>
-cudaError_t run(const KernelParams &kp, const Plan &plan, cudaStream_t stream) {
+cudaError_t run(const KernelParams &kp, const Plan &plan, int sms, cudaStream_t stream) {
   using C = Cfg<kKind, DP, NT>;
   auto kernel = decode_attention_kernel<kKind, DP, NT>;
   static std::atomic<uint64_t> ready{0};  // one bit per device
@@ -1049,24 +1064,31 @@ cudaError_t run(const KernelParams &kp, const Plan &plan, cudaStream_t stream) {
   fp.join_parts = tiles < plan.grid;
   fp.join_blocks = plan.joins_needed ? (uint32_t)(fp.join_parts ? tiles : plan.grid) * (pieces / fp.pieces) : 0;
   uint64_t blocks = fp.join_blocks;
-  if (kp.logits) blocks += (uint64_t)((kp.cap + kWeightTokens - 1) / kWeightTokens) * kp.a.c.n_heads * kp.a.c.batch;
+  if (kp.logits) {
+    // a block finds its heads' log-sum-exps first: chunks long enough that the blocks are few waves
+    const uint64_t heads = (uint64_t)kp.a.c.n_heads * kp.a.c.batch;
+    uint64_t chunk = kWeightTokens;
+    while (chunk < kp.cap && heads * ((kp.cap + chunk - 1) / chunk) > 4ull * sms) chunk *= 2;
+    fp.weight_chunk = (uint32_t)chunk;
+    blocks += heads * ((kp.cap + chunk - 1) / chunk);
+  }
   if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidValue;
   if (blocks)
-    e = launch_after(finish_kernel<DP, NT, kKind == kKindE4m3>, dim3((unsigned)blocks), dim3(256), kp.logits ? 4ull * kp.group : 0, stream, fp);
+    e = launch_after(finish_kernel<DP, NT, kKind == kKindE4m3>, dim3((unsigned)blocks), dim3(256), kp.logits ? 4ull * (kp.group + 3) : 0, stream, fp);
   return e;
 }
 
 template <int kKind, int DP>
-cudaError_t run_group(const KernelParams &kp, const Plan &plan, cudaStream_t stream) {
-  return plan.tile_heads == 8 ? run<kKind, DP, 1>(kp, plan, stream) : run<kKind, DP, 2>(kp, plan, stream);
+cudaError_t run_group(const KernelParams &kp, const Plan &plan, int sms, cudaStream_t stream) {
+  return plan.tile_heads == 8 ? run<kKind, DP, 1>(kp, plan, sms, stream) : run<kKind, DP, 2>(kp, plan, sms, stream);
 }
 
 template <int kKind>
-cudaError_t run_dim(const KernelParams &kp, const Plan &plan, cudaStream_t stream) {
+cudaError_t run_dim(const KernelParams &kp, const Plan &plan, int sms, cudaStream_t stream) {
   switch (padded_dim(kp.a.c.head_dim)) {
-    case 64: return run_group<kKind, 64>(kp, plan, stream);
-    case 128: return run_group<kKind, 128>(kp, plan, stream);
-    default: return run_group<kKind, 256>(kp, plan, stream);
+    case 64: return run_group<kKind, 64>(kp, plan, sms, stream);
+    case 128: return run_group<kKind, 128>(kp, plan, sms, stream);
+    default: return run_group<kKind, 256>(kp, plan, sms, stream);
   }
 }
 
@@ -1095,9 +1117,9 @@ cudaError_t launch_decode_attention(const DecodeAttentionParams &a, int sms, cud
     kp.lse2 = reinterpret_cast<float *>(a.workspace + plan.lse2);
     kp.logits = reinterpret_cast<float *>(a.workspace + plan.logits);
   }
-  if (a.c.dtype == kE4m3) return run_dim<kKindE4m3>(kp, plan, stream);
-  if (a.c.dtype == kFp16) return run_dim<kKindFp16>(kp, plan, stream);
-  return run_dim<kKindBf16>(kp, plan, stream);
+  if (a.c.dtype == kE4m3) return run_dim<kKindE4m3>(kp, plan, sms, stream);
+  if (a.c.dtype == kFp16) return run_dim<kKindFp16>(kp, plan, sms, stream);
+  return run_dim<kKindBf16>(kp, plan, sms, stream);
 }
 
 }  // namespace kvs
