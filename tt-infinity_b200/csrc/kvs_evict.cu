@@ -54,9 +54,10 @@ __device__ __forceinline__ uint32_t length_of(const EvictParams &p, uint32_t b) 
 // digits of the keys, most significant first: 10, 8, 8 and 6 bits
 constexpr uint32_t kAllBins = 1024 + 256 + 256 + 64;
 constexpr uint32_t kNoBin = 0xFFFFFFFFu;
+constexpr uint32_t kFew = kSelThreads;  // keys that are ranked against one another, one per thread
 
 struct Found {
-  uint32_t bin, left, total;
+  uint32_t bin, left, count, total;  // count: keys in the bin
 };
 
 // Exclusive prefix of `mine` over the threads' warps (what the warps before this one hold) and the sum
@@ -115,12 +116,13 @@ __device__ Found find_bin(cg::cluster_group &cluster, uint32_t *hist, uint32_t w
       if (above < goal && goal <= above + bins[i]) {
         s_out[0] = low + i;
         s_out[1] = goal - above;
+        s_out[2] = bins[i];
       }
       above += bins[i];
     }
   }
   __syncthreads();
-  return Found{s_out[0], s_out[1], w.y};
+  return Found{s_out[0], s_out[1], s_out[2], w.y};
 }
 
 // Page of slot i of request b's destination, or -1.
@@ -184,7 +186,9 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   __shared__ __align__(16) uint32_t s_hist[kAllBins];
   __shared__ uint32_t s_count[2];           // above the threshold, equal to it
   __shared__ uint32_t s_warp[6][kSelWarps];
-  __shared__ uint32_t s_out[4][2];
+  __shared__ uint32_t s_out[5][3];
+  __shared__ __align__(16) uint32_t s_all[kFew];
+  __shared__ uint32_t s_few[kFew], s_few_count;
   __shared__ MoveRows s_rows;
   cg::cluster_group cluster = cg::this_cluster();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -206,7 +210,8 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   auto key_at = [&](uint32_t i) -> uint32_t { return cached ? s_keys[i] : key_from(i, __ldg(w + t0 + i), __ldg(table + p.page.quotient(t0 + i))); };
 
   for (uint32_t i = tid; i < kAllBins; i += kSelThreads) s_hist[i] = 0;
-  if (tid < 4) s_out[tid][0] = kNoBin;
+  if (tid < 5) s_out[tid][0] = kNoBin;
+  if (tid == 0) s_few_count = 0;
   __syncthreads();
   constexpr uint32_t kAhead = 8;
   for (uint32_t base = tid; base < n; base += kSelThreads * kAhead) {
@@ -240,21 +245,66 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     }
     cluster.sync();
   };
+  // Few keys share the digits found: every CTA collects them all and ranks each against the others.
+  auto rank_few = [&](uint32_t low, uint32_t wanted, uint32_t total) {
+    for (uint32_t i = tid; i < n; i += kSelThreads) {
+      const uint32_t key = key_at(i);
+      if (key && (key ^ found) >> low == 0) s_few[atomicAdd(&s_few_count, 1u)] = key;
+    }
+    cluster.sync();
+    const uint32_t theirs = lane < ctas ? *cluster.map_shared_rank(&s_few_count, lane) : 0;
+    uint32_t before = 0, mine = 0;
+    bool here = false;
+    for (uint32_t r = 0; r < ctas; ++r) {
+      const uint32_t count = __shfl_sync(~0u, theirs, r);
+      if (tid >= before && tid < before + count) {
+        mine = cluster.map_shared_rank(s_few, r)[tid - before];
+        here = true;
+      }
+      before += count;
+    }
+    s_all[tid] = here ? mine : 0;  // zeros behind the last one count for nothing
+    __syncthreads();
+    if (here) {
+      uint32_t larger = 0, same = 0;
+#pragma unroll 4
+      for (uint32_t i = 0; i < total; i += 4) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(s_all + i);
+        larger += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+        same += (x.x == mine) + (x.y == mine) + (x.z == mine) + (x.w == mine);
+      }
+      if (larger < wanted && wanted <= larger + same) {
+        s_out[4][0] = mine;
+        s_out[4][1] = wanted - larger;
+      }
+    }
+    __syncthreads();
+    found = s_out[4][0];
+    left = s_out[4][1];
+  };
   if (f.bin != kNoBin) {
     found = f.bin << 22;
-    next_digit(s_hist + 1024, 14, 8);
-    f = find_bin<256>(cluster, s_hist + 1024, f.left, s_warp[1], s_out[1]);
-    if (f.bin != kNoBin) {
-      found |= f.bin << 14;
-      next_digit(s_hist + 1280, 6, 8);
-      f = find_bin<256>(cluster, s_hist + 1280, f.left, s_warp[2], s_out[2]);
+    if (f.count <= kFew) {
+      rank_few(22, f.left, f.count);
+    } else {
+      next_digit(s_hist + 1024, 14, 8);
+      f = find_bin<256>(cluster, s_hist + 1024, f.left, s_warp[1], s_out[1]);
       if (f.bin != kNoBin) {
-        found |= f.bin << 6;
-        next_digit(s_hist + 1536, 0, 6);
-        f = find_bin<64>(cluster, s_hist + 1536, f.left, s_warp[3], s_out[3]);
-        if (f.bin != kNoBin) {
-          found |= f.bin;
-          left = f.left;
+        found |= f.bin << 14;
+        if (f.count <= kFew) {
+          rank_few(14, f.left, f.count);
+        } else {
+          next_digit(s_hist + 1280, 6, 8);
+          f = find_bin<256>(cluster, s_hist + 1280, f.left, s_warp[2], s_out[2]);
+          if (f.bin != kNoBin) {
+            found |= f.bin << 6;
+            next_digit(s_hist + 1536, 0, 6);
+            f = find_bin<64>(cluster, s_hist + 1536, f.left, s_warp[3], s_out[3]);
+            if (f.bin != kNoBin) {
+              found |= f.bin;
+              left = f.left;
+            }
+          }
         }
       }
     }
@@ -309,7 +359,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     for (uint32_t i = begin + tid; i < end; i += kSelThreads) w_out[i] = in_turn ? __uint_as_float(s_keys[i - begin]) : __ldg(w + kept[i]);
     for (uint32_t i = want + rank * kSelThreads + tid; i < len; i += ctas * kSelThreads) w_out[i] = 0.f;
   }
-  if (p.dst_table) move_rows(p, b, h, kept, begin, end, s_rows);
+  if (p.dst_table && !p.move_apart) move_rows(p, b, h, kept, begin, end, s_rows);
 }
 
 constexpr int kMoveThreads = 256;
@@ -340,6 +390,16 @@ __global__ void __launch_bounds__(kMoveThreads) move_weights_kernel(const __grid
   }
   __syncthreads();
   for (uint32_t i = n + threadIdx.x; i < len; i += kMoveThreads) o[i] = 0.f;
+}
+
+// To fresh pages, in a launch of its own: kMoveApart ranks of one (request, head) per CTA.
+constexpr uint32_t kMoveApart = 64;
+__global__ void __launch_bounds__(kSelThreads) move_kernel(const __grid_constant__ EvictParams p) {
+  __shared__ MoveRows s_rows;
+  const uint32_t h = blockIdx.y, b = blockIdx.z;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint32_t begin = blockIdx.x * kMoveApart, end = min((uint32_t)p.new_lens[b], begin + kMoveApart);
+  if (begin < end) move_rows(p, b, h, p.kept + ((uint64_t)b * p.c.n_heads + h) * p.keep, begin, end, s_rows);
 }
 
 // In place: one CTA moves a 64-byte column of K (even blockIdx.x) or V of one (request, head),
@@ -415,7 +475,12 @@ cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   at[0].val.clusterDim = {ctas, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, select_kernel, p, cached);
+  EvictParams q = p;
+#ifndef TUNE_APART
+#define TUNE_APART (rows * ctas < 2ull * sms)
+#endif
+  q.move_apart = p.dst_table && TUNE_APART;
+  e = cudaLaunchKernelEx(&cfg, select_kernel, q, cached);
   if (e != cudaSuccess) return e;
   count_launch();
   // the move starts while the selection drains and waits for its results itself
@@ -423,6 +488,14 @@ cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kMoveThreads);
   cfg.dynamicSmemBytes = 0;
+  if (q.move_apart) {
+    const uint64_t most = cap < p.keep ? cap : p.keep;
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.gridDim = dim3((unsigned)((most + kMoveApart - 1) / kMoveApart), p.c.n_heads, p.c.batch);
+    e = cudaLaunchKernelEx(&cfg, move_kernel, p);
+    if (e != cudaSuccess) return e;
+    count_launch();
+  }
   if (!p.dst_table) {
     cfg.gridDim = dim3(2 * ((p.row_bytes + 63) / 64), p.c.n_heads, p.c.batch);
     e = cudaLaunchKernelEx(&cfg, move_in_place_kernel, p);
