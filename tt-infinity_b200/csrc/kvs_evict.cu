@@ -125,62 +125,7 @@ __device__ Found find_bin(cg::cluster_group &cluster, uint32_t *hist, uint32_t w
   return Found{s_out[0], s_out[1], s_out[2], w.y};
 }
 
-// Page of slot i of request b's destination, or -1.
-__device__ __forceinline__ int32_t dst_page(const EvictParams &p, uint32_t b, uint32_t vb) {
-  if (vb >= p.dst_blocks) return -1;
-  const int32_t pg = __ldg(p.dst_table + (uint64_t)b * p.dst_blocks + vb);
-  return pg > 0 && (uint32_t)pg < p.c.num_blocks ? pg : -1;
-}
-
-// Where a batch of kept rows comes from and goes to, as byte offsets into K and V; -1: nowhere.
-constexpr uint32_t kMoveRows = 128;
-struct MoveRows {
-  int64_t k_src[kMoveRows], v_src[kMoveRows], k_dst[kMoveRows], v_dst[kMoveRows];
-};
-
-// Rows of the kept tokens of ranks [begin, end) to their slots on fresh pages, by the whole CTA.
-__device__ void move_rows(const EvictParams &p, uint32_t b, uint32_t h, const int32_t *kept, uint32_t begin, uint32_t end, MoveRows &s) {
-  const uint32_t tid = threadIdx.x, words = p.row_bytes / 16;
-  for (uint32_t base = begin; base < end; base += kMoveRows) {
-    const uint32_t rows = min(kMoveRows, end - base);
-    __syncthreads();
-    for (uint32_t r = tid; r < rows; r += kSelThreads) {
-      const uint32_t i = base + r, t = (uint32_t)kept[i];
-      const uint32_t sb = p.page.quotient(t), db = p.page.quotient(i), sr = p.page.rest(t, sb), dr = p.page.rest(i, db);
-      const int32_t sp = page_of(p.c, b, sb), dp = dst_page(p, b, db);
-      s.k_src[r] = (int64_t)sp * p.c.k_page + (int64_t)h * p.c.k_head + (int64_t)sr * p.c.k_row;
-      s.v_src[r] = (int64_t)sp * p.c.v_page + (int64_t)h * p.c.v_head + (int64_t)sr * p.c.v_row;
-      s.k_dst[r] = dp < 0 ? -1 : (int64_t)dp * p.c.k_page + (int64_t)h * p.c.k_head + (int64_t)dr * p.c.k_row;
-      s.v_dst[r] = dp < 0 ? -1 : (int64_t)dp * p.c.v_page + (int64_t)h * p.c.v_head + (int64_t)dr * p.c.v_row;
-      if (dp < 0 && h == 0 && p.out_of_range) atomicAdd(p.out_of_range, 1u);
-    }
-    __syncthreads();
-    const uint32_t side = rows * words;
-    constexpr int kAhead = 4;  // rows' words in flight per thread, of K and of V
-    for (uint32_t at = tid; at < side; at += kSelThreads * kAhead) {
-      int4 x[kAhead], y[kAhead];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const uint32_t e = at + u * kSelThreads, r = p.words.quotient(e), q = p.words.rest(e, r);
-        if (e < side) {
-          x[u] = *reinterpret_cast<const int4 *>(p.c.k + s.k_src[r] + 16 * q);
-          y[u] = *reinterpret_cast<const int4 *>(p.c.v + s.v_src[r] + 16 * q);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const uint32_t e = at + u * kSelThreads, r = p.words.quotient(e), q = p.words.rest(e, r);
-        if (e < side && s.k_dst[r] >= 0) {
-          *reinterpret_cast<int4 *>(p.c.k + s.k_dst[r] + 16 * q) = x[u];
-          *reinterpret_cast<int4 *>(p.c.v + s.v_dst[r] + 16 * q) = y[u];
-        }
-      }
-    }
-  }
-}
-
-// Chooses the tokens of one (request, KV head) per cluster and moves what a CTA chose of its tokens:
-// their weights, and their rows where they go to fresh pages.
+// Chooses the tokens of one (request, KV head) per cluster and moves their weights.
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_constant__ EvictParams p, uint32_t cached_keys) {
   extern __shared__ __align__(16) uint32_t s_keys[];
   __shared__ __align__(16) uint32_t s_hist[kAllBins];
@@ -189,47 +134,76 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   __shared__ uint32_t s_out[5][3];
   __shared__ __align__(16) uint32_t s_all[kFew];
   __shared__ uint32_t s_few[kFew], s_few_count;
-  __shared__ MoveRows s_rows;
   cg::cluster_group cluster = cg::this_cluster();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const uint32_t row = blockIdx.x / ctas, b = row / p.c.n_heads, h = row % p.c.n_heads;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t len = length_of(p, b);
-  const uint32_t piece = (len + ctas - 1) / ctas;
+  const uint32_t piece = ((len + ctas - 1) / ctas + 3) / 4 * 4;  // tokens are taken four at a time
   const uint32_t t0 = min(len, rank * piece), n = min(len - t0, piece);
   const float *w = p.weights + (int64_t)b * p.w_req + (int64_t)h * p.w_head;
   const bool cached = piece <= cached_keys;
 
-  // key of this CTA's token i from its weight and its page-table entry
   const int32_t *table = p.c.page_table + (uint64_t)b * p.c.max_blocks;
-  auto key_from = [&](uint32_t i, float x, int32_t page) -> uint32_t {
-    const uint32_t t = t0 + i, key = t < p.first || t + p.recent >= len ? kStays : key_of(x);
-    return page > 0 && (uint32_t)page < p.c.num_blocks ? key : 0u;
+  const uint32_t quads = (n + 3) / 4;
+  // four weights, and their pages (one, where four tokens never lie in two): loads only
+  auto load_quad = [&](uint32_t q, float4 &x, int4 &page) {
+    const uint32_t t = t0 + 4 * q;
+    if (p.vector_weights && 4 * q + 3 < n) {
+      x = __ldg(reinterpret_cast<const float4 *>(w + t));
+    } else {
+      x.x = __ldg(w + t);
+      x.y = __ldg(w + min(t + 1, len - 1));
+      x.z = __ldg(w + min(t + 2, len - 1));
+      x.w = __ldg(w + min(t + 3, len - 1));
+    }
+    page.x = __ldg(table + p.page.quotient(t));
+    if (p.c.block_size % 4 == 0) {
+      page.y = page.z = page.w = page.x;
+    } else {
+      page.y = __ldg(table + p.page.quotient(min(t + 1, len - 1)));
+      page.z = __ldg(table + p.page.quotient(min(t + 2, len - 1)));
+      page.w = __ldg(table + p.page.quotient(min(t + 3, len - 1)));
+    }
   };
-  auto key_at = [&](uint32_t i) -> uint32_t { return cached ? s_keys[i] : key_from(i, __ldg(w + t0 + i), __ldg(table + p.page.quotient(t0 + i))); };
+  auto keys_of = [&](uint32_t q, const float4 &x, const int4 &page) -> uint4 {
+    auto key = [&](uint32_t i, float y, int32_t pg) -> uint32_t {
+      const uint32_t t = t0 + i;
+      const bool there = pg > 0 && (uint32_t)pg < p.c.num_blocks && i < n;
+      return !there ? 0u : (t < p.first || t + p.recent >= len ? kStays : key_of(y));
+    };
+    return make_uint4(key(4 * q, x.x, page.x), key(4 * q + 1, x.y, page.y), key(4 * q + 2, x.z, page.z), key(4 * q + 3, x.w, page.w));
+  };
+  auto quad_at = [&](uint32_t q) -> uint4 {
+    if (cached) return reinterpret_cast<const uint4 *>(s_keys)[q];
+    float4 x;
+    int4 page;
+    load_quad(q, x, page);
+    return keys_of(q, x, page);
+  };
 
   for (uint32_t i = tid; i < kAllBins; i += kSelThreads) s_hist[i] = 0;
   if (tid < 5) s_out[tid][0] = kNoBin;
   if (tid == 0) s_few_count = 0;
   __syncthreads();
-  constexpr uint32_t kAhead = 8;
-  for (uint32_t base = tid; base < n; base += kSelThreads * kAhead) {
-    float x[kAhead];
-    int32_t page[kAhead];
+  constexpr uint32_t kAhead = 4;
+  for (uint32_t base = tid; base < quads; base += kSelThreads * kAhead) {
+    float4 x[kAhead];
+    int4 page[kAhead];
 #pragma unroll
-    for (uint32_t u = 0; u < kAhead; ++u) {  // all on their way before the first is looked at
-      const uint32_t t = t0 + min(base + u * kSelThreads, n - 1);
-      x[u] = __ldg(w + t);
-      page[u] = __ldg(table + p.page.quotient(t));
-    }
+    for (uint32_t u = 0; u < kAhead; ++u)  // all on their way before the first is looked at
+      load_quad(min(base + u * kSelThreads, quads - 1), x[u], page[u]);
 #pragma unroll
     for (uint32_t u = 0; u < kAhead; ++u) {
-      const uint32_t i = base + u * kSelThreads;
-      if (i >= n) break;
-      const uint32_t key = key_from(i, x[u], page[u]);
-      if (cached) s_keys[i] = key;
-      if (key) atomicAdd(&s_hist[key >> 22], 1u);
+      const uint32_t q = base + u * kSelThreads;
+      if (q >= quads) break;
+      const uint4 k = keys_of(q, x[u], page[u]);
+      if (cached) reinterpret_cast<uint4 *>(s_keys)[q] = k;
+      if (k.x) atomicAdd(&s_hist[k.x >> 22], 1u);
+      if (k.y) atomicAdd(&s_hist[k.y >> 22], 1u);
+      if (k.z) atomicAdd(&s_hist[k.z >> 22], 1u);
+      if (k.w) atomicAdd(&s_hist[k.w >> 22], 1u);
     }
   }
   cluster.sync();
@@ -238,18 +212,27 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   // keys above `found` are chosen, and the first `left` equal to it; where all keys of a bin are
   // wanted, its lowest key is as good a threshold as any (and with no bin at all the lowest key, 1)
   uint32_t found = 0, left = kNoBin;
+  // (no key below 2^22 but 0 has a token, so keys that share the first digit are tokens' keys)
   auto next_digit = [&](uint32_t *hist, uint32_t shift, uint32_t bits) {
-    for (uint32_t i = tid; i < n; i += kSelThreads) {
-      const uint32_t key = key_at(i);
-      if (key && (key ^ found) >> (shift + bits) == 0) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
+    auto count = [&](uint32_t key) {
+      if ((key ^ found) >> (shift + bits) == 0) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
+    };
+#pragma unroll 2
+    for (uint32_t q = tid; q < quads; q += kSelThreads) {
+      const uint4 k = quad_at(q);
+      count(k.x), count(k.y), count(k.z), count(k.w);
     }
     cluster.sync();
   };
   // Few keys share the digits found: every CTA collects them all and ranks each against the others.
   auto rank_few = [&](uint32_t low, uint32_t wanted, uint32_t total) {
-    for (uint32_t i = tid; i < n; i += kSelThreads) {
-      const uint32_t key = key_at(i);
-      if (key && (key ^ found) >> low == 0) s_few[atomicAdd(&s_few_count, 1u)] = key;
+    auto collect = [&](uint32_t key) {
+      if ((key ^ found) >> low == 0) s_few[atomicAdd(&s_few_count, 1u)] = key;
+    };
+#pragma unroll 2
+    for (uint32_t q = tid; q < quads; q += kSelThreads) {
+      const uint4 k = quad_at(q);
+      collect(k.x), collect(k.y), collect(k.z), collect(k.w);
     }
     cluster.sync();
     const uint32_t theirs = lane < ctas ? *cluster.map_shared_rank(&s_few_count, lane) : 0;
@@ -311,14 +294,18 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   }
   found = max(found, 1u);
   // chosen: keys above `found`, and the first `left` keys equal to it
-  const uint32_t share = ((n + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
-  const uint32_t i0 = min(n, warp * share), i1 = min(n, i0 + share);
+  const uint32_t share = ((quads + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;  // quads of a warp
+  const uint32_t q0 = min(quads, warp * share), q1 = min(quads, q0 + share);
+  auto above_in = [&](const uint4 &k) { return (uint32_t)(k.x > found) + (k.y > found) + (k.z > found) + (k.w > found); };
+  auto equal_in = [&](const uint4 &k) { return (uint32_t)(k.x == found) + (k.y == found) + (k.z == found) + (k.w == found); };
   uint32_t above = 0, equal = 0;
-  for (uint32_t i = i0; i < i1; i += 32) {
-    const uint32_t key = i + lane < i1 ? key_at(i + lane) : 0;
-    above += __popc(__ballot_sync(~0u, key > found));
-    equal += __popc(__ballot_sync(~0u, key == found));
+  for (uint32_t q = q0 + lane; q < q1; q += 32) {
+    const uint4 k = quad_at(q);
+    above += above_in(k);
+    equal += equal_in(k);
   }
+  above = __reduce_add_sync(~0u, above);
+  equal = __reduce_add_sync(~0u, equal);
   const uint2 of_above = over_warps(above, s_warp[4]), of_equal = over_warps(equal, s_warp[5]);
   uint32_t cta_above = 0, cta_equal = 0;  // in the CTAs before this one
   if (ctas > 1) {
@@ -336,14 +323,29 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   above = cta_above + of_above.x;
   equal = cta_equal + of_equal.x;
   int32_t *kept = p.kept + (uint64_t)row * p.keep;
-  for (uint32_t i = i0; i < i1; i += 32) {
-    const uint32_t key = i + lane < i1 ? key_at(i + lane) : 0;
-    const uint32_t ba = __ballot_sync(~0u, key > found), be = __ballot_sync(~0u, key == found);
-    const uint32_t below = (1u << lane) - 1;
-    const uint32_t a = above + __popc(ba & below), e = equal + __popc(be & below);
-    if (key > found || (key == found && e < left)) kept[a + min(e, left)] = (int32_t)(t0 + i + lane);
-    above += __popc(ba);
-    equal += __popc(be);
+  for (uint32_t base = q0; base < q1; base += 32) {  // the warp's quads in order
+    const uint32_t q = base + lane;
+    const uint4 k = q < q1 ? quad_at(q) : make_uint4(0, 0, 0, 0);
+    const uint32_t own = above_in(k) | equal_in(k) << 16;
+    uint32_t incl = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += y;
+    }
+    uint32_t a = above + ((incl - own) & 0xFFFFu), e = equal + ((incl - own) >> 16);
+    auto place = [&](uint32_t key, uint32_t i) {
+      if (key > found) {
+        kept[a + min(e, left)] = (int32_t)(t0 + i);
+        ++a;
+      } else if (key == found) {
+        if (e < left) kept[a + e] = (int32_t)(t0 + i);
+        ++e;
+      }
+    };
+    place(k.x, 4 * q), place(k.y, 4 * q + 1), place(k.z, 4 * q + 2), place(k.w, 4 * q + 3);
+    const uint32_t all = __shfl_sync(~0u, incl, 31);
+    above += all & 0xFFFFu;
+    equal += all >> 16;
   }
   for (uint32_t i = want + rank * kSelThreads + tid; i < p.keep; i += ctas * kSelThreads) kept[i] = -1;
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = (int32_t)want;
@@ -359,7 +361,6 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     for (uint32_t i = begin + tid; i < end; i += kSelThreads) w_out[i] = in_turn ? __uint_as_float(s_keys[i - begin]) : __ldg(w + kept[i]);
     for (uint32_t i = want + rank * kSelThreads + tid; i < len; i += ctas * kSelThreads) w_out[i] = 0.f;
   }
-  if (p.dst_table && !p.move_apart) move_rows(p, b, h, kept, begin, end, s_rows);
 }
 
 constexpr int kMoveThreads = 256;
@@ -392,14 +393,56 @@ __global__ void __launch_bounds__(kMoveThreads) move_weights_kernel(const __grid
   for (uint32_t i = n + threadIdx.x; i < len; i += kMoveThreads) o[i] = 0.f;
 }
 
-// To fresh pages, in a launch of its own: kMoveApart ranks of one (request, head) per CTA.
-constexpr uint32_t kMoveApart = 64;
-__global__ void __launch_bounds__(kSelThreads) move_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ MoveRows s_rows;
-  const uint32_t h = blockIdx.y, b = blockIdx.z;
+// Page of slot i of request b's destination, or -1.
+__device__ __forceinline__ int32_t dst_page(const EvictParams &p, uint32_t b, uint32_t vb) {
+  if (vb >= p.dst_blocks) return -1;
+  const int32_t pg = __ldg(p.dst_table + (uint64_t)b * p.dst_blocks + vb);
+  return pg > 0 && (uint32_t)pg < p.c.num_blocks ? pg : -1;
+}
+
+// To fresh pages: kMoveRows ranks of one (request, head) per CTA.
+constexpr uint32_t kMoveRows = 64;
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ EvictParams p) {
+  __shared__ struct {
+    int64_t k_src[kMoveRows], v_src[kMoveRows], k_dst[kMoveRows], v_dst[kMoveRows];  // byte offsets; -1: nowhere
+  } s;
+  const uint32_t h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, words = p.row_bytes / 16;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const uint32_t begin = blockIdx.x * kMoveApart, end = min((uint32_t)p.new_lens[b], begin + kMoveApart);
-  if (begin < end) move_rows(p, b, h, p.kept + ((uint64_t)b * p.c.n_heads + h) * p.keep, begin, end, s_rows);
+  const uint32_t n = (uint32_t)p.new_lens[b], base = blockIdx.x * kMoveRows;
+  if (base >= n) return;
+  const uint32_t rows = min(kMoveRows, n - base);
+  if (tid < rows) {
+    const uint32_t i = base + tid, t = (uint32_t)p.kept[((uint64_t)b * p.c.n_heads + h) * p.keep + i];
+    const uint32_t sb = p.page.quotient(t), db = p.page.quotient(i), sr = p.page.rest(t, sb), dr = p.page.rest(i, db);
+    const int32_t sp = page_of(p.c, b, sb), dp = dst_page(p, b, db);
+    s.k_src[tid] = (int64_t)sp * p.c.k_page + (int64_t)h * p.c.k_head + (int64_t)sr * p.c.k_row;
+    s.v_src[tid] = (int64_t)sp * p.c.v_page + (int64_t)h * p.c.v_head + (int64_t)sr * p.c.v_row;
+    s.k_dst[tid] = dp < 0 ? -1 : (int64_t)dp * p.c.k_page + (int64_t)h * p.c.k_head + (int64_t)dr * p.c.k_row;
+    s.v_dst[tid] = dp < 0 ? -1 : (int64_t)dp * p.c.v_page + (int64_t)h * p.c.v_head + (int64_t)dr * p.c.v_row;
+    if (dp < 0 && h == 0 && p.out_of_range) atomicAdd(p.out_of_range, 1u);
+  }
+  __syncthreads();
+  const uint32_t side = rows * words;
+  constexpr int kAhead = 4;  // words in flight per thread, of K and of V
+  for (uint32_t at = tid; at < side; at += kMoveThreads * kAhead) {
+    int4 x[kAhead], y[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t e = at + u * kMoveThreads, r = p.words.quotient(e), q = p.words.rest(e, r);
+      if (e < side) {
+        x[u] = *reinterpret_cast<const int4 *>(p.c.k + s.k_src[r] + 16 * q);
+        y[u] = *reinterpret_cast<const int4 *>(p.c.v + s.v_src[r] + 16 * q);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t e = at + u * kMoveThreads, r = p.words.quotient(e), q = p.words.rest(e, r);
+      if (e < side && s.k_dst[r] >= 0) {
+        *reinterpret_cast<int4 *>(p.c.k + s.k_dst[r] + 16 * q) = x[u];
+        *reinterpret_cast<int4 *>(p.c.v + s.v_dst[r] + 16 * q) = y[u];
+      }
+    }
+  }
 }
 
 // In place: one CTA moves a 64-byte column of K (even blockIdx.x) or V of one (request, head),
@@ -451,8 +494,8 @@ cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   // rows of up to 32768 tokens: 92 us with four CTAs per row, 98 us with eight.)
   const uint64_t rows = (uint64_t)p.c.batch * p.c.n_heads;
   uint32_t ctas = 1;
-  while (ctas < 8 && cap > 1024ull * ctas && (rows * ctas < 2ull * sms || cap > 8192ull * ctas)) ctas *= 2;
-  const uint64_t piece = (cap + ctas - 1) / ctas;
+  while (ctas < 8 && cap > 1024ull * ctas && (rows * ctas < 1ull * sms || cap > 8192ull * ctas)) ctas *= 2;
+  const uint64_t piece = ((cap + ctas - 1) / ctas + 3) / 4 * 4;
   const uint32_t cached = piece <= kMaxCached ? (uint32_t)piece : 0;
   const size_t smem = 4ull * cached;
   static std::atomic<uint64_t> ready{0};  // one bit per device
@@ -476,10 +519,7 @@ cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   cfg.attrs = at;
   cfg.numAttrs = 1;
   EvictParams q = p;
-#ifndef TUNE_APART
-#define TUNE_APART (rows * ctas < 2ull * sms)
-#endif
-  q.move_apart = p.dst_table && TUNE_APART;
+  q.vector_weights = (reinterpret_cast<uintptr_t>(p.weights) & 15) == 0 && p.w_req % 4 == 0 && p.w_head % 4 == 0;
   e = cudaLaunchKernelEx(&cfg, select_kernel, q, cached);
   if (e != cudaSuccess) return e;
   count_launch();
@@ -488,10 +528,9 @@ cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kMoveThreads);
   cfg.dynamicSmemBytes = 0;
-  if (q.move_apart) {
+  if (p.dst_table) {
     const uint64_t most = cap < p.keep ? cap : p.keep;
-    cfg.blockDim = dim3(kSelThreads);
-    cfg.gridDim = dim3((unsigned)((most + kMoveApart - 1) / kMoveApart), p.c.n_heads, p.c.batch);
+    cfg.gridDim = dim3((unsigned)((most + kMoveRows - 1) / kMoveRows), p.c.n_heads, p.c.batch);
     e = cudaLaunchKernelEx(&cfg, move_kernel, p);
     if (e != cudaSuccess) return e;
     count_launch();

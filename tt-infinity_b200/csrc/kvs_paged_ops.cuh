@@ -111,7 +111,7 @@ struct EvictParams {
   uint32_t row_bytes;
   Divisor page;               // block_size
   Divisor words;              // 16-byte words of a row
-  bool move_apart;            // rows go to fresh pages in a launch of their own
+  bool vector_weights;        // rows of weights start on 16-byte boundaries
 };
 cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream);
 
