@@ -83,7 +83,7 @@ def check_attend(seed, lens, *, dtype=BF16, cache="same", dim=128, heads=2, grou
     bad = np.abs(got - out) > b_out
     assert not bad.any(), (np.abs(got - out)[bad].max(), b_out[bad].min(), np.argwhere(bad)[:4])
     empty = np.isinf(lse)
-    assert (got_lse[empty] == -np.inf).all() and (np.abs(got_lse - lse)[~empty] <= b_lse[~empty]).all()
+    assert (got_lse[empty] == -np.inf).all() and (np.abs(got_lse[~empty] - lse[~empty]) <= b_lse[~empty]).all()
     if weights:
         gw = R.f64(args["weights_out"])
         for b, n in enumerate(lens):
@@ -166,6 +166,15 @@ def test_attention_strides_and_given_output():
     assert torch.equal(out, ref) and (store[..., :dim] == 0).all()
     assert (wbuf[:, heads] == 0).all()
     assert torch.allclose(wbuf[:, :heads].sum(2), torch.full((2, heads), float(group), device="cuda"), atol=1e-4)
+
+
+def test_attention_reads_broadcast_heads():
+    g = gen(19)
+    k, v, table = cache_of(g, [70], 16, 1, 64, BF16)
+    q = torch.randn((1, 4, 64), generator=g).to(BF16).cuda()
+    one = ops.paged_decode_attention(q, k.cuda(), v.cuda(), i32(table), i32([70]))
+    two = ops.paged_decode_attention(q, k.cuda().expand(-1, 2, -1, -1), v.cuda().expand(-1, 2, -1, -1), i32(table), i32([70]))
+    assert torch.allclose(one.float(), two.float(), atol=2.0**-7)
 
 
 def test_attention_nan_and_infinite_values_reach_only_their_row():
@@ -377,12 +386,12 @@ def test_fill_no_tokens():
 
 
 def check_evict(seed, lens, keep, *, first=0, recent=0, heads=2, dim=64, page=16, layout="hnd", dtype=BF16, in_place=False,
-                holes=(), ties=True):
+                holes=(), ties=True, extra=5):
     g = gen(seed)
     k, v, table = cache_of(g, lens, page, heads, dim, dtype, holes=holes, spare=2 + sum(-(-min(n, keep) // page) for n in lens))
     blocks = k.shape[0]
     cover = table.shape[1] * page
-    w = torch.rand((len(lens), heads, cover + 5), generator=g)
+    w = torch.rand((len(lens), heads, cover + extra), generator=g)
     if ties:
         w = (w * 8).floor() / 4 - 0.5
         w[torch.rand(w.shape, generator=g) < 0.05] = -0.0
@@ -439,6 +448,13 @@ def test_evict_layouts(dim, page, layout, dtype, in_place):
 
 
 @pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens,keep", [([3, 4, 5, 97], 4), ([900, 2050, 0, 1023], 300), ([6001], 2500)])
+def test_evict_weights_on_16_byte_rows(lens, keep, in_place):
+    check_evict(keep, lens, keep, first=1, recent=2, in_place=in_place, page=16, dim=16, extra=0)
+    check_evict(keep, lens, keep, first=1, recent=2, in_place=in_place, page=18, dim=16, extra=(-(max(lens) // 18 + 2) * 18) % 4, ties=False)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
 def test_evict_missing_pages(in_place):
     holes = {(0, 0), (0, 1), (0, 2), (1, 1), (1, 3), (2, 0)}
     check_evict(21, [45, 100, 90, 50], 30, first=5, recent=10, holes=holes, in_place=in_place)
@@ -458,13 +474,18 @@ def test_evict_row_longer_than_a_cluster_holds():
     w = torch.rand((1, 1, page * 98), generator=g).cuda()
     table = i32(np.concatenate([np.arange(1, 99)])[None])
     ck, cv = (torch.zeros((100, 1, page, 8), dtype=BF16, device="cuda") for _ in range(2))
-    kept, lens = ops.evict_paged_kv(ck, cv, table, i32([n]), w, 1000, first=2, recent=3, dst_page_table=i32([[99]]),
-                                    weights_out=w.clone())
+    old = w.clone()
+    kept, lens = ops.evict_paged_kv(ck, cv, table, i32([n]), w, 1000, first=2, recent=3, dst_page_table=i32([[99]]))
+    after, w = w, old
+    other = torch.full_like(w, 5)
+    again, _ = ops.evict_paged_kv(ck, cv, table, i32([n]), w, 1000, first=2, recent=3, dst_page_table=i32([[99]]), weights_out=other)
     key = w[0, 0, :n].clone()
     key[:2] = 9
     key[-3:] = 9
     want = torch.sort(torch.sort(key, descending=True, stable=True).indices[:1000]).values
-    assert int(lens[0]) == 1000 and torch.equal(kept[0, 0].long(), want)
+    assert int(lens[0]) == 1000 and torch.equal(kept[0, 0].long(), want) and torch.equal(again, kept)
+    assert torch.equal(after[0, 0, :1000], w[0, 0, want]) and (after[0, 0, 1000:n] == 0).all() and torch.equal(after[0, 0, n:], w[0, 0, n:])
+    assert torch.equal(other[0, 0, :n], after[0, 0, :n]) and (other[0, 0, n:] == 5).all()
 
 
 # ------------------------------------------------------------------ a run of them, streams, graphs
@@ -612,7 +633,8 @@ def test_refusals():
                         (dict(positions=n(2, 8)), "need axes"), (dict(positions=n(7)), "positions must be"),
                         (dict(positions=n(2, 8), axes=n(31)), "rotary / 2"), (dict(axes=n(32)), "only with positions"),
                         (dict(positions=n(33, 8), axes=n(32)), "32 axes"), (dict(eps=-1.0), "eps"), (dict(q_out=z(8, 4, 32)), "q_out"),
-                        (dict(out_of_range=z(1)), "int32"), (dict(q=z(8, 4, 64).requires_grad_()), "no backward")]:
+                        (dict(out_of_range=z(1)), "int32"), (dict(q_out=z(1, 4, 64).expand(8, 4, 64)), "broadcast"),
+                        (dict(cache_v=z(1, 2, 16, 64).expand(4, 2, 16, 64)), "broadcast"), (dict(q=z(8, 4, 64).requires_grad_()), "no backward")]:
         with pytest.raises(RuntimeError, match=msg):
             ops.qk_norm_rope_fill(**dict(fill, **change))
     att = dict(q=z(2, 4, 64), cache_k=z(4, 2, 16, 64), cache_v=z(4, 2, 16, 64), page_table=n(2, 2), seq_lens=n(2))
@@ -620,7 +642,8 @@ def test_refusals():
     f32 = lambda *s: z(*s, dt=torch.float32)
     for change, msg in [(dict(q=z(3, 4, 64)), "requests"), (dict(q=z(2, 3, 64)), "multiple of the KV heads"), (dict(seq_lens=n(3)), "must match"),
                         (dict(seq_lens=f32(2)), "INT32"), (dict(window=0), "window"), (dict(scale=float("nan")), "scale"),
-                        (dict(out=z(2, 4, 32)), "out must"), (dict(weights=f32(2, 2, 31)), "must cover"), (dict(weights=f32(2, 4, 32)), "num_kv_heads"),
+                        (dict(out=z(2, 4, 32)), "out must"), (dict(out=z(2, 1, 64).expand(2, 4, 64)), "broadcast"),
+                        (dict(weights=f32(2, 1, 32).expand(2, 2, 32)), "broadcast"), (dict(weights=f32(2, 2, 31)), "must cover"), (dict(weights=f32(2, 4, 32)), "num_kv_heads"),
                         (dict(weights_out=f32(2, 2, 32)), "needs weights"), (dict(q=z(2, 4, 64, dt=torch.float32)), "rows must be"),
                         (dict(cache_k=z(4, 2, 16, 512), cache_v=z(4, 2, 16, 512), q=z(2, 4, 512)), "up to 256"),
                         (dict(cache_k=z(4, 2, 16, 24, dt=E4M3), cache_v=z(4, 2, 16, 24, dt=E4M3), q=z(2, 4, 24)), "multiple of 16"),
@@ -631,7 +654,8 @@ def test_refusals():
     ops.evict_paged_kv(**ev)
     for change, msg in [(dict(keep=0), "keep"), (dict(first=5, recent=4), "first"), (dict(recent=-1), "recent"), (dict(weights=f32(2, 2, 30)), "must cover"),
                         (dict(dst_page_table=n(1, 1)), "batch_size"), (dict(dst_page_table=n(2, 1), keep=17), "must cover keep"),
-                        (dict(weights_out=f32(2, 2, 16)), "must cover"), (dict(seq_lens=n(1)), "must match")]:
+                        (dict(weights_out=f32(2, 2, 16)), "must cover"), (dict(cache_k=z(4, 1, 16, 64).expand(4, 2, 16, 64)), "broadcast"),
+                        (dict(seq_lens=n(1)), "must match")]:
         with pytest.raises(RuntimeError, match=msg):
             ops.evict_paged_kv(**dict(ev, **change))
 

@@ -44,24 +44,31 @@ def test_rows_checks():
     lib = _native.load()
     assert "null" in error(lib.kvs_paged_decode_attention(C.byref(cache()), None, None))
     assert "null" in error(lib.kvs_paged_decode_attention(None, None, None))
-    d = lambda **kw: C.byref(_native.DecodeRows(**dict(dict(q=P16, out=P16, q_heads=4, dtype=0, scale=1.0), **kw)))
+    two = (C.c_int64 * 2)(512, 128)
+    d = lambda **kw: C.byref(_native.DecodeRows(**dict(dict(q=P16, out=P16, q_heads=4, dtype=0, scale=1.0, out_strides=two, weights_out_strides=two), **kw)))
     attend = lambda **kw: error(lib.kvs_paged_decode_attention(C.byref(cache()), d(**kw), None))
     assert "same type" in attend(dtype=1) and "bf16 or fp16" in attend(dtype=2) and "multiple of the KV heads" in attend(q_heads=3)
     assert "16-byte" in attend(q=P16 + 2) and "finite" in attend(scale=float("inf")) and "go together" in attend(weights=P16)
     assert "must cover" in attend(weights=P16, weights_out=P16, w_len=31) and "256-byte" in attend(workspace=P16 + 16)
     assert "1024" in attend(q_heads=4096)
+    flat = (C.c_int64 * 2)(512, 0)
+    assert "broadcast" in attend(out_strides=flat) and "broadcast" in attend(weights=P16, weights_out=P16, w_len=32, weights_out_strides=flat)
     assert "must be on device" in attend()  # host addresses are refused, not read
     f = lambda **kw: C.byref(_native.QkvRows(**dict(dict(q=P16, k=P16, v=P16, q_out=P16, cos_sin=P16, q_heads=4, rotary=64,
-                                                         n_positions=8, n_tokens=1), **kw)))
+                                                         n_positions=8, n_tokens=2, q_out_strides=two), **kw)))
     fill = lambda **kw: error(lib.kvs_qk_norm_rope_fill(C.byref(cache()), f(**kw), None))
     assert "rotary" in fill(rotary=72) and "rotary" in fill(rotary=4) and "at least one row" in fill(n_positions=0)
     assert "eps" in fill(eps=-1.0) and "16-byte" in fill(q_weight=P16 + 4) and "axes" in fill(axes=P16) and "axes" in fill(positions=P16)
+    assert "broadcast" in fill(q_out_strides=flat)
     assert "must be on device" in fill()
     assert lib.kvs_qk_norm_rope_fill(C.byref(cache()), f(n_tokens=0), None) == 0
-    e = lambda **kw: C.byref(_native.EvictRows(**dict(dict(keep=8, w_len=32, wo_len=32), **kw)))
+    e = lambda **kw: C.byref(_native.EvictRows(**dict(dict(keep=8, w_len=32, wo_len=32, weights_strides=two, weights_out_strides=two), **kw)))
     evict = lambda **kw: error(lib.kvs_evict_paged(C.byref(cache()), e(**kw), None))
     assert "keep" in evict(keep=0) and "first (5)" in evict(first=5, recent=4) and "must cover keep" in evict(dst_table=P16)
     assert "must cover" in evict(w_len=31) and "must cover" in evict(wo_len=31) and "must be on device" in evict()
+    assert "broadcast" in evict(weights_out_strides=flat) and "not overlap" in evict(weights=P16, weights_out=P16, weights_strides=(C.c_int64 * 2)(8, 4))
+    single = cache(k_strides=(C.c_int64 * 3)(4096, 0, 128))
+    assert "broadcast" in error(lib.kvs_evict_paged(C.byref(single), e(), None)) and "broadcast" in error(lib.kvs_qk_norm_rope_fill(C.byref(single), f(), None))
 
 
 def test_cpu_tensors_are_refused():

@@ -7,18 +7,24 @@
 //
 // What bounds it: every valid K and V row is read once; the arithmetic is 2 * group flop per cache
 // byte (16-bit cache), far below what the tensor cores do in the time the bytes take, so the kernel
-// is built to keep loads in flight:
+// is built to keep loads in flight and instructions few:
 //   * Each warp streams its own 16-token tiles of K and V through a private ring in shared memory
 //     (16-byte cp.async, zero-filled where a token is masked, so that nothing a masked slot holds
-//     -- infinities, NaN -- reaches the sums). No CTA barrier stands in the main loop.
+//     -- infinities, NaN -- reaches the sums). No CTA barrier stands in the main loop, and the loads
+//     run ahead of the products across the ends of requests and heads.
 //   * The products run with the tokens as the rows of the matrix instruction: S^T = K Q^T
 //     (16 tokens x 8 heads) and O^T = V^T P^T (16 elements x 8 heads), so a group of up to 8 heads
 //     fills the 8 columns and no instruction works on padding rows; groups up to 16 take two column
-//     tiles and larger ones several passes over the cache.
-//   * Work is split by tokens, not by request: the batch's tiles, in units of kUnitTiles, form one
+//     tiles and larger ones several passes over the cache. (Memory is the bound: the tensor pipe is
+//     busy 8 % of the time for a bf16 cache, 16 % for e4m3.)
+//   * Work is split by tokens, not by request: the batch's tiles, in units of a few tiles, form one
 //     sequence that is cut into equal runs, one per CTA, from lengths that only the device knows.
 //     A (request, head) that spans several CTAs leaves partial sums that a second small kernel
 //     joins, in the order of the sequence, so results do not depend on timing.
+// Device times, with the share of the measured copy rate: 48 contexts up to 16384 tokens, 8 KV heads of
+// 128, group 8, bf16: 233 us, 100 %; one of 131071: 89 us, 93 %; 64 up to 12001 from an e4m3 cache: 168 us,
+// 81 % (token-major pages of 16: a head's rows are 128 bytes in every 1024), 143 us, 95 % from head-major
+// pages.
 //
 // Scores, maxima, sums and accumulators are 32-bit. The probabilities are rounded to the cache's
 // 16-bit type for the second product (fp16 for an e4m3 cache): each is off by at most half a step,
@@ -38,40 +44,30 @@ namespace kvs {
 
 namespace {
 
-#ifndef TUNE_WARPS
-#define TUNE_WARPS 4
-#endif
-constexpr int kWarps = TUNE_WARPS;
+constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr uint32_t kTile = 16;       // tokens per warp tile
-#ifndef TUNE_UNIT
-#define TUNE_UNIT 4
-#define TUNE_LEAST 4
-#define TUNE_WHOLE 512
-#endif
+constexpr uint32_t kTile = 16;  // tokens per warp tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 enum Kind { kKindBf16, kKindFp16, kKindE4m3 };
 
-// How a kernel streams: 16-token tiles per step, steps in the ring, bytes of a warp's ring and CTAs
-// per SM, by bytes per element, padded head_dim and column tiles of 8 heads.
+// How a kernel streams: tiles in a warp's ring, bytes of a CTA's rings and CTAs per SM, by bytes per
+// element, padded head_dim and column tiles of 8 heads. Rows of up to 128 bytes carry few bytes per
+// instruction, so they get more warps where registers allow: 3 CTAs per SM with 64 KiB each (e4m3, head_dim 128, 64 mixed contexts up to 12001 tokens:
+// 168 us against 171 us with 4 CTAs of 48 KiB and 172 us with 2 of 96 KiB). Longer rows take 2 CTAs of
+// 96 KiB, and rows of 512 bytes one of 192 KiB, three tiles per warp being the least that keeps loads
+// in flight while a tile is worked on.
 struct Shape {
-  int sub, stages, ring, ctas;
+  int stages, ring, ctas;
 };
-#ifndef TUNE_SUB
-#define TUNE_SUB (el == 2 && dp == 64 && nt == 1 ? 2 : 1)
-#define TUNE_BYTES (el == 1 && dp * nt <= 128 && nt == 1 ? 49152 : dp == 64 && nt == 2 ? 65536 : 98304)
-#define TUNE_CTAS (el == 1 && dp * nt <= 128 && nt == 1 ? 4 : dp == 64 && nt == 2 ? 3 : 2)
-#endif
 __host__ __device__ constexpr Shape shape_of(int el, int dp, int nt) {
   Shape s{};
-  s.sub = TUNE_SUB;
-  const int stage = 2 * 16 * s.sub * dp * el;
-  const int fit = TUNE_BYTES / (kWarps * stage);
+  const bool light = dp * el <= 128 && dp * nt <= 128;
+  const int stage = 2 * 16 * dp * el, fit = (light ? 65536 : 98304) / (kWarps * stage);
   s.stages = fit < 3 ? 3 : (fit > 8 ? 8 : fit);
   s.ring = kWarps * s.stages * stage;
-  s.ctas = s.ring > 110 * 1024 ? 1 : TUNE_CTAS;
+  s.ctas = s.ring > 110 * 1024 ? 1 : (light ? 3 : 2);
   return s;
 }
 
@@ -81,9 +77,7 @@ struct Cfg {
   static constexpr Shape shape = shape_of(el, DP, NT);
   static constexpr int pitch = DP * el;                 // bytes of a row in shared memory
   static constexpr int chunks = pitch / 16;             // 16-byte pieces of a row
-  static constexpr int sub = shape.sub;
-  static constexpr uint32_t tokens = 16 * sub;
-  static constexpr int stage = 2 * (int)tokens * pitch; // K and V of one step
+  static constexpr int stage = 2 * (int)kTile * pitch;  // K and V of one tile
   static constexpr int stages = shape.stages;
   static constexpr int ring = shape.ring;
   static constexpr int ctas = shape.ctas;
@@ -118,15 +112,22 @@ Plan plan_of(const PagedCache &c, uint32_t q_heads, bool weights, int sms) {
   const uint32_t per_sm = shape_of(c.dtype == kE4m3 ? 1 : 2, dp, p.tile_heads / 8).ctas;
   const uint64_t cap = (uint64_t)c.max_blocks * c.block_size;
   const uint32_t cap_tiles = (uint32_t)((cap + kTile - 1) / kTile);
-  const bool whole = cap <= TUNE_WHOLE;
-  p.unit_tiles = whole ? cap_tiles : TUNE_UNIT;
-  p.least_units = whole ? 1 : TUNE_LEAST;
+  // Runs are cut at units of 64 tokens, and a CTA takes 128 tokens at least where requests are at most
+  // 2048 tokens long, else 256: shorter runs leave more parts to join (one request, one KV head, 32768
+  // tokens: 13.8 us, with 128 tokens at least 19.4 us; one request of 1024 tokens, 8 heads: 9.5 us with
+  // 256, 8.5 us with 128). Short requests are not cut at all, which saves the join: 2 requests of up to
+  // 193 tokens 7.2 us against 9.1 us, 16 of up to 300 8.0 us against 11.1 us; but one of 500 tokens, 8
+  // heads, 9.8 us against 7.7 us, so above 256 tokens only where the GPU has enough of them.
+  const uint64_t tiles = (uint64_t)c.batch * c.n_heads * p.head_tiles;
+  const bool whole = cap <= 256 || (cap <= 512 && 4 * tiles >= (uint64_t)sms);
+  p.unit_tiles = whole ? cap_tiles : 4;
+  p.least_units = whole ? 1 : (cap <= 2048 ? 2 : 4);
   const uint64_t units = (cap_tiles + p.unit_tiles - 1) / p.unit_tiles;
-  const uint64_t most = ((uint64_t)c.batch * c.n_heads * p.head_tiles * units + p.least_units - 1) / p.least_units;
+  const uint64_t most = (tiles * units + p.least_units - 1) / p.least_units;
   const uint64_t full = (uint64_t)sms * per_sm;
   p.grid = (uint32_t)(most < full ? most : full);
   p.joins_needed = units > 1 && p.grid > 1;
-  p.narrow = c.batch <= kThreads && (uint64_t)c.batch * c.n_heads * p.head_tiles * units < 1ull << 31;
+  p.narrow = c.batch <= kThreads && tiles * units < 1ull << 31;
   uint64_t off = 0;
   auto take = [&](uint64_t n) {
     const uint64_t o = off;
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
   uint8_t *const smem = smem_raw + (-smem_addr(smem_raw) & 511);
   __shared__ uint64_t s_scan[kWarps];
   __shared__ Cursor s_at;
-  __shared__ uint32_t s_mask[kWarps][C::stages][C::sub];
+  __shared__ uint32_t s_mask[kWarps][C::stages];
   __shared__ float s_m[C::heads], s_l[C::heads];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedCache &c = p.a.c;
@@ -398,47 +399,42 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
     }
   };
   // ---- loads
-  constexpr uint32_t stride = kWarps * C::sub;  // tiles between a warp's steps
-  uint32_t load_tile_at = ahead.begin(p) + warp * C::sub, load_end = ahead.end(p);
-  int32_t pages[C::sub];  // of the tiles of the next step to load; 0: masked
-  uint32_t slots[C::sub]; // this lane's token's (the tile's first token's) slot in its page
-  const uint8_t *kh, *vh; // this KV head's rows; this lane's piece of them where a tile lies in one page
+  uint32_t load_tile_at = ahead.begin(p) + warp, load_end = ahead.end(p);
+  int32_t page;            // of the next tile to load; 0: masked
+  uint32_t slot;           // this lane's token's (the tile's first token's) slot in its page
+  const uint8_t *kh, *vh;  // this KV head's rows; this lane's piece of them where a tile lies in one page
   auto find_head = [&]() {
     const uint32_t h = ahead.hh / p.head_tiles;
     kh = c.k + (int64_t)h * c.k_head + my_chunk * 16;
     vh = c.v + (int64_t)h * c.v_head + my_chunk * 16;
   };
-  auto find_pages = [&]() {
-#pragma unroll
-    for (int u = 0; u < C::sub; ++u) {
-      pages[u] = 0;
-      slots[u] = 0;
-      const uint32_t tile = load_tile_at + u;
-      if (tile >= load_end) continue;
-      // page of this lane's token (of the whole tile, where it lies in one page)
-      const uint32_t t = tile * kTile + (one_page ? 0 : (lane & 15)), vb = p.page.quotient(t);
-      slots[u] = p.page.rest(t, vb);
-      if (vb >= c.max_blocks) continue;
-      const int32_t pg = __ldg(c.page_table + (uint64_t)ahead.b * c.max_blocks + vb);
-      pages[u] = pg > 0 && (uint32_t)pg < c.num_blocks ? pg : 0;
-    }
+  auto find_page = [&]() {
+    page = 0;
+    slot = 0;
+    if (load_tile_at >= load_end) return;
+    // page of this lane's token (of the whole tile, where it lies in one page)
+    const uint32_t t = load_tile_at * kTile + (one_page ? 0 : (lane & 15)), vb = p.page.quotient(t);
+    slot = p.page.rest(t, vb);
+    if (vb >= c.max_blocks) return;
+    const int32_t pg = __ldg(c.page_table + (uint64_t)ahead.b * c.max_blocks + vb);
+    page = pg > 0 && (uint32_t)pg < c.num_blocks ? pg : 0;
   };
-  // to the next step of this warp, through runs that have none for it
+  // to the next tile of this warp, through runs that have none for it
   auto settle = [&]() {
     while (load_tile_at >= load_end && ahead.left) {
       ahead.next(p, hh_n);
       if (!ahead.left) break;
-      load_tile_at = ahead.begin(p) + warp * C::sub;
+      load_tile_at = ahead.begin(p) + warp;
       load_end = ahead.end(p);
       find_head();
     }
-    if (ahead.left) find_pages();
+    if (ahead.left) find_page();
   };
   // one tile of K and V into shared memory, and which of its tokens count
-  auto load_tile = [&](uint32_t tile, uint32_t kdst, uint32_t vdst, int32_t page, uint32_t slot, uint32_t *note) {
-    const uint32_t t0 = tile * kTile;
-    uint32_t mask = tile < load_end ? 0xFFFFu : 0u;
-    if (t0 + kTile > ahead.span.len && mask) mask = 0xFFFFu >> min(16u, t0 + kTile - ahead.span.len);
+  auto load_tile = [&](uint32_t kdst, uint32_t vdst, uint32_t *note) {
+    const uint32_t t0 = load_tile_at * kTile;
+    uint32_t mask = 0xFFFFu;
+    if (t0 + kTile > ahead.span.len) mask = 0xFFFFu >> (t0 + kTile - ahead.span.len);
     if (t0 < ahead.span.low) mask &= 0xFFFFu << (ahead.span.low - t0);
     if (one_page) mask = page ? mask : 0;
     else mask &= __ballot_sync(~0u, page != 0);
@@ -475,14 +471,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
       }
     }
   };
-  // one step's loads; past the last step the group is empty, so that groups keep counting
+  // one tile's loads; past the last one the group is empty, so that groups keep counting
   auto issue = [&](uint32_t stage) {
     if (ahead.left) {
-      const uint32_t kdst = ring + stage * C::stage, vdst = kdst + C::tokens * C::pitch;
-#pragma unroll
-      for (int u = 0; u < C::sub; ++u)
-        load_tile(load_tile_at + u, kdst + u * kTile * C::pitch, vdst + u * kTile * C::pitch, pages[u], slots[u], &s_mask[warp][stage][u]);
-      load_tile_at += stride;
+      const uint32_t kdst = ring + stage * C::stage;
+      load_tile(kdst, kdst + kTile * C::pitch, &s_mask[warp][stage]);
+      load_tile_at += kWarps;
       settle();
     }
     cp_commit();
@@ -490,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
   // Rows shorter than the padded head_dim: the products run over zeros behind them, which no load
   // overwrites.
   if (row_chunks < C::chunks)
-    for (uint32_t row = lane; row < C::stages * 2 * C::tokens; row += 32)
+    for (uint32_t row = lane; row < C::stages * 2 * kTile; row += 32)
       for (uint32_t j = row_chunks; j < C::chunks; ++j)
         *reinterpret_cast<uint4 *>(smem + warp * C::stages * C::stage + row * C::pitch + ((j ^ swizzle(row)) << 4)) = make_uint4(0, 0, 0, 0);
   find_head();
@@ -557,69 +551,57 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
         for (int i = 0; i < 4; ++i) acc[nt][s][i] = 0.f;
     }
 
-    for (uint32_t tile = t_begin + warp * C::sub; tile < t_end; tile += stride) {
+    for (uint32_t tile = t_begin + warp; tile < t_end; tile += kWarps) {
       cp_wait<C::stages - 2>();
       __syncwarp();
       issue(stage == 0 ? C::stages - 1 : stage - 1);
-      const uint32_t kt = ring + stage * C::stage + k_place, vt = ring + stage * C::stage + C::tokens * C::pitch + v_place;
+      const uint32_t kt = ring + stage * C::stage + k_place, vt = ring + stage * C::stage + kTile * C::pitch + v_place;
 
-      // ---- S^T = K Q^T (two chains of products per tile)
-      float sc[C::sub][NT][4];
+      // ---- S^T = K Q^T (two chains of products)
+      float sc[NT][4];
       {
-        float sd[C::sub][NT][4];
+        float sd[NT][4];
 #pragma unroll
-        for (int u = 0; u < C::sub; ++u)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[u][nt][i] = sd[u][nt][i] = 0.f;
+          for (int i = 0; i < 4; ++i) sc[nt][i] = sd[nt][i] = 0.f;
 #pragma unroll
         for (int s = 0; s < kSteps; s += 2) {
+          uint32_t a[4];
+          if (!k8) {
+            ldsm4(a, kt ^ (uint32_t)(s << 5));
 #pragma unroll
-          for (int u = 0; u < C::sub; ++u) {
-            const uint32_t at = kt + u * kTile * C::pitch;
-            if (!k8) {
-              uint32_t a[4];
-              ldsm4(a, at ^ (s << 5));
+            for (int nt = 0; nt < NT; ++nt) mma<kBf>(sc[nt], a[0], a[1], a[2], a[3], bq[s][nt][0], bq[s][nt][1]);
+            ldsm4(a, kt ^ (uint32_t)((s + 1) << 5));
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma<kBf>(sc[u][nt], a[0], a[1], a[2], a[3], bq[s][nt][0], bq[s][nt][1]);
-              ldsm4(a, at ^ ((s + 1) << 5));
+            for (int nt = 0; nt < NT; ++nt) mma<kBf>(sd[nt], a[0], a[1], a[2], a[3], bq[s + 1][nt][0], bq[s + 1][nt][1]);
+          } else {
+            ldsm4(a, kt ^ (uint32_t)(s << 4));
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma<kBf>(sd[u][nt], a[0], a[1], a[2], a[3], bq[s + 1][nt][0], bq[s + 1][nt][1]);
-            } else {
-              uint32_t a[4];
-              ldsm4(a, at ^ (s << 4));
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t x0 = widen(a[2 * i]), x1 = widen(a[2 * i + 1]), x2 = widen(a[2 * i] >> 16), x3 = widen(a[2 * i + 1] >> 16);
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t x0 = widen(a[2 * i]), x1 = widen(a[2 * i + 1]), x2 = widen(a[2 * i] >> 16), x3 = widen(a[2 * i + 1] >> 16);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma<false>(i ? sd[u][nt] : sc[u][nt], x0, x1, x2, x3, bq[s + i][nt][0], bq[s + i][nt][1]);
-              }
+              for (int nt = 0; nt < NT; ++nt) mma<false>(i ? sd[nt] : sc[nt], x0, x1, x2, x3, bq[s + i][nt][0], bq[s + i][nt][1]);
             }
           }
         }
 #pragma unroll
-        for (int u = 0; u < C::sub; ++u)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[u][nt][i] = (sc[u][nt][i] + sd[u][nt][i]) * head_scale[nt][i & 1];
+          for (int i = 0; i < 4; ++i) sc[nt][i] = (sc[nt][i] + sd[nt][i]) * head_scale[nt][i & 1];
       }
 
-      // ---- running maximum and sum; tokens lane / 4 and lane / 4 + 8 of each tile, heads 2j and 2j + 1
+      // ---- running maximum and sum; tokens lane / 4 and lane / 4 + 8, heads 2j and 2j + 1
+      const uint32_t mask = s_mask[warp][stage];
+      if (mask != 0xFFFFu) {
+        const bool in0 = (mask >> (lane >> 2)) & 1, in1 = (mask >> ((lane >> 2) + 8)) & 1;
 #pragma unroll
-      for (int u = 0; u < C::sub; ++u) {
-        const uint32_t mask = s_mask[warp][stage][u];
-        if (mask != 0xFFFFu) {
-          const bool in0 = (mask >> (lane >> 2)) & 1, in1 = (mask >> ((lane >> 2) + 8)) & 1;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              if (!in0) sc[u][nt][i] = -INFINITY;
-              if (!in1) sc[u][nt][2 + i] = -INFINITY;
-            }
-        }
+          for (int i = 0; i < 2; ++i) {
+            if (!in0) sc[nt][i] = -INFINITY;
+            if (!in1) sc[nt][2 + i] = -INFINITY;
+          }
       }
       bool grew = false;
       float mn[NT][2];
@@ -627,9 +609,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float x = fmaxf(sc[0][nt][i], sc[0][nt][2 + i]);
-#pragma unroll
-          for (int u = 1; u < C::sub; ++u) x = fmaxf(x, fmaxf(sc[u][nt][i], sc[u][nt][2 + i]));
+          float x = fmaxf(sc[nt][i], sc[nt][2 + i]);
           x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
           x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
           x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
@@ -637,25 +617,22 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
           grew |= mn[nt][i] > m[nt][i];
         }
       if (p.logits) {
+        const uint32_t t = tile * kTile + (lane >> 2);
+        float *lg = p.logits + (((uint64_t)b * c.n_heads + h) * p.cap + t) * p.group + g0;
 #pragma unroll
-        for (int u = 0; u < C::sub; ++u) {
-          const uint32_t t = (tile + u) * kTile + (lane >> 2);
-          float *lg = p.logits + (((uint64_t)b * c.n_heads + h) * p.cap + t) * p.group + g0;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t g = nt * 8 + 2 * (lane & 3);
-              if (t + 8 * i >= at.span.len || g >= heads) continue;
-              float *to = lg + 8ull * i * p.group + g;
-              if (p.group % 2 == 0) {
-                *reinterpret_cast<float2 *>(to) = make_float2(sc[u][nt][2 * i], sc[u][nt][2 * i + 1]);
-              } else {
-                to[0] = sc[u][nt][2 * i];
-                if (g + 1 < heads) to[1] = sc[u][nt][2 * i + 1];
-              }
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t g = nt * 8 + 2 * (lane & 3);
+            if (t + 8 * i >= at.span.len || g >= heads) continue;
+            float *to = lg + 8ull * i * p.group + g;
+            if (p.group % 2 == 0) {
+              *reinterpret_cast<float2 *>(to) = make_float2(sc[nt][2 * i], sc[nt][2 * i + 1]);
+            } else {
+              to[0] = sc[nt][2 * i];
+              if (g + 1 < heads) to[1] = sc[nt][2 * i + 1];
             }
-        }
+          }
       }
       if (__any_sync(~0u, grew)) {
 #pragma unroll
@@ -672,47 +649,40 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
             }
           }
       }
-      uint32_t pb[C::sub][NT][2];
+      uint32_t pb[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float base0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], base1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-#pragma unroll
-        for (int u = 0; u < C::sub; ++u) {
-          const float e0 = exp2_fast(sc[u][nt][0] - base0), e1 = exp2_fast(sc[u][nt][1] - base1);
-          const float e2 = exp2_fast(sc[u][nt][2] - base0), e3 = exp2_fast(sc[u][nt][3] - base1);
-          l[nt][0] += e0 + e2;
-          l[nt][1] += e1 + e3;
-          pb[u][nt][0] = transpose8(pack2<kBf>(e0, e1));
-          pb[u][nt][1] = transpose8(pack2<kBf>(e2, e3));
-        }
+        const float e0 = exp2_fast(sc[nt][0] - base0), e1 = exp2_fast(sc[nt][1] - base1);
+        const float e2 = exp2_fast(sc[nt][2] - base0), e3 = exp2_fast(sc[nt][3] - base1);
+        l[nt][0] += e0 + e2;
+        l[nt][1] += e1 + e3;
+        pb[nt][0] = transpose8(pack2<kBf>(e0, e1));
+        pb[nt][1] = transpose8(pack2<kBf>(e2, e3));
       }
 
       // ---- O^T += V^T P^T
+      if (!k8) {
 #pragma unroll
-      for (int u = 0; u < C::sub; ++u) {
-        const uint32_t at = vt + u * kTile * C::pitch;
-        if (!k8) {
+        for (int s = 0; s < kSteps; ++s) {
+          uint32_t a[4];
+          ldsm4t(a, vt ^ (uint32_t)(s << 5));
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            uint32_t a[4];
-            ldsm4t(a, at ^ (s << 5));
+          for (int nt = 0; nt < NT; ++nt) mma<kBf>(acc[nt][s], a[0], a[1], a[2], a[3], pb[nt][0], pb[nt][1]);
+        }
+      } else {
+        // a transposed load of byte pairs gives (t0 d0, t0 d1, t1 d0, t1 d1): even elements become
+        // rows 0-7 of the 16-element tile, odd ones rows 8-15
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma<kBf>(acc[nt][s], a[0], a[1], a[2], a[3], pb[u][nt][0], pb[u][nt][1]);
-          }
-        } else {
-          // a transposed load of byte pairs gives (t0 d0, t0 d1, t1 d0, t1 d1): even elements become
-          // rows 0-7 of the 16-element tile, odd ones rows 8-15
+        for (int s = 0; s < kSteps; s += 2) {
+          uint32_t a[4];
+          ldsm4t(a, vt ^ (uint32_t)(s << 4));
 #pragma unroll
-          for (int s = 0; s < kSteps; s += 2) {
-            uint32_t a[4];
-            ldsm4t(a, at ^ (s << 4));
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t lo = __byte_perm(a[i], 0, 0x3120), hi = __byte_perm(a[2 + i], 0, 0x3120);
+            const uint32_t x0 = widen(lo), x1 = widen(lo >> 16), x2 = widen(hi), x3 = widen(hi >> 16);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t lo = __byte_perm(a[i], 0, 0x3120), hi = __byte_perm(a[2 + i], 0, 0x3120);
-              const uint32_t x0 = widen(lo), x1 = widen(lo >> 16), x2 = widen(hi), x3 = widen(hi >> 16);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma<false>(acc[nt][s + i], x0, x1, x2, x3, pb[u][nt][0], pb[u][nt][1]);
-            }
+            for (int nt = 0; nt < NT; ++nt) mma<false>(acc[nt][s + i], x0, x1, x2, x3, pb[nt][0], pb[nt][1]);
           }
         }
       }
@@ -734,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
     // ---- warp 0 takes in the other warps' sums, one after the other (those that had a step)
     float4 *const buf = reinterpret_cast<float4 *>(smem + C::ring);
     for (uint32_t w = 1; w < kWarps; ++w) {
-      if (t_begin + w * C::sub >= t_end) break;
+      if (t_begin + w >= t_end) break;
       if (warp == w) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {

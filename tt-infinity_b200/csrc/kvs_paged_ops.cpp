@@ -103,6 +103,15 @@ int check_cache(const kvs_paged_cache *c, const char *op, kvs::PagedCache *out) 
   return KVS_OK;
 }
 
+// Dimensions of what a call writes: none of several elements may have stride 0 (a broadcast view).
+bool spread(const int64_t *strides, uint64_t n0, uint64_t n1) { return (n0 <= 1 || strides[0]) && (n1 <= 1 || strides[1]); }
+int check_written(const kvs_paged_cache *c, const char *op) {
+  CHECK(spread(c->k_strides, c->num_blocks, c->n_heads) && spread(c->v_strides, c->num_blocks, c->n_heads) &&
+            (c->block_size <= 1 || (c->k_strides[2] && c->v_strides[2])),
+        "%s: cache_k and cache_v must not be broadcast", op);
+  return KVS_OK;
+}
+
 int check_row_type(int32_t dtype, int32_t cache, const char *op) {
   CHECK(dtype == KVS_DTYPE_BF16 || dtype == KVS_DTYPE_FP16, "%s: rows must be bf16 or fp16", op);
   CHECK(cache == KVS_DTYPE_E4M3 || cache == dtype, "%s: rows and cache must have the same type (or the cache e4m3)", op);
@@ -151,6 +160,8 @@ int kvs_qk_norm_rope_fill(const kvs_paged_cache *cache, const kvs_qkv_rows *r, v
   CHECK(aligned16(r->cos_sin) && aligned16(r->q_weight) && aligned16(r->k_weight) && aligned16(r->axes),
         "%s: cos_sin, axes and weights must start on 16-byte boundaries", op);
   CHECK(std::isfinite(r->eps) && r->eps >= 0, "%s: eps must be finite and not negative", op);
+  TRY(check_written(cache, op));
+  CHECK(spread(r->q_out_strides, r->n_tokens, r->q_heads), "%s: q_out must not be broadcast", op);
   if (r->n_tokens == 0) return KVS_OK;
   Where w{op};
   TRY(add_cache(w, cache));
@@ -215,6 +226,8 @@ int kvs_paged_decode_attention(const kvs_paged_cache *cache, const kvs_decode_ro
   CHECK(aligned16(r->q) && aligned16(r->out) && strides16(r->q_strides, 2) && strides16(r->out_strides, 2),
         "%s: q and out rows must start on 16-byte boundaries", op);
   CHECK(std::isfinite(r->scale), "%s: scale must be finite", op);
+  CHECK(spread(r->out_strides, cache->batch, r->q_heads), "%s: out must not be broadcast", op);
+  CHECK(!r->weights_out || spread(r->weights_out_strides, cache->batch, cache->n_heads), "%s: weights_out must not be broadcast", op);
   CHECK((r->weights == nullptr) == (r->weights_out == nullptr), "%s: weights and weights_out go together", op);
   CHECK(!r->weights || r->w_len >= (uint64_t)cache->max_blocks * cache->block_size,
         "%s: weights must cover max_num_blocks_per_seq * block_size tokens", op);
@@ -261,6 +274,8 @@ int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *r, void 
   kvs::EvictParams p{};
   TRY(check_cache(cache, op, &p.c));
   CHECK(r, "%s: the rows are null", op);
+  TRY(check_written(cache, op));
+  CHECK(spread(r->weights_out_strides, cache->batch, cache->n_heads), "%s: weights_out must not be broadcast", op);
   CHECK(r->keep > 0 && r->keep <= 0x7FFFFFFFu, "%s: keep must be 1 to 2^31 - 1", op);
   CHECK((uint64_t)r->first + r->recent <= r->keep, "%s: first (%u) + recent (%u) must be <= keep (%u)", op, r->first,
         r->recent, r->keep);
