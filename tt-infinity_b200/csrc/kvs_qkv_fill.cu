@@ -223,20 +223,31 @@ __global__ void __launch_bounds__(32) qkv_fill_kernel(const __grid_constant__ Qk
   // the first rows are on their way while the token's place is looked up
   R::load(x, in, row0, end, w, lo, hi);
   if (!is_q) R::load(v, p.v_head, row0, end, w, v_lo, v_hi);
+  // and so is what does not depend on that place
+  uint32_t pos = p.positions && lane < p.n_axes ? (uint32_t)__ldg(p.positions + (uint64_t)lane * p.tokens + t) : 0;
+  int4 axis[PP / 4] = {};
+  if (p.axes && w.turns)
+#pragma unroll
+    for (int i = 0; i < PP / 4; ++i) axis[i] = __ldg(reinterpret_cast<const int4 *>(p.axes + w.pair) + i);
+  const void *weight = is_q ? p.q_weight : p.k_weight;
+  typename R::H weight_lo, weight_hi;
+  if (weight && w.mine) {
+    weight_lo = __ldg(reinterpret_cast<const typename R::H *>(static_cast<const uint8_t *>(weight) + 2 * w.e0));
+    weight_hi = __ldg(reinterpret_cast<const typename R::H *>(static_cast<const uint8_t *>(weight) + 2 * w.e1));
+  }
 
   // ---- the token: its request, its slot in the cache and its position
   const uint32_t upto = entries_up_to(p.cu_seqlens, c.batch + 1, t, lane);
   const bool inside = upto >= 1 && upto <= c.batch && (uint32_t)__ldg(p.cu_seqlens + upto) != 0xFFFFFFFFu;
   bool bad = false;
-  uint32_t slot = 0, pos = 0, vb = 0;
+  uint32_t slot = 0, vb = 0;
   int32_t page = 0;
   if (inside) {
     const uint32_t req = upto - 1;
     slot = t - (uint32_t)__ldg(p.cu_seqlens + req) + (uint32_t)__ldg(p.start + req);
     vb = slot < 0x80000000u ? p.page.quotient(slot) : c.max_blocks;
     page = page_of(c, req, vb);
-    pos = slot;
-    if (p.positions) pos = lane < p.n_axes ? (uint32_t)__ldg(p.positions + (uint64_t)lane * p.tokens + t) : 0;
+    if (!p.positions) pos = slot;
     bad = __any_sync(~0u, pos >= p.n_positions);
     if ((bad || page < 0) && blockIdx.y == 0 && lane == 0 && p.out_of_range) atomicAdd(p.out_of_range, 1u);
   }
@@ -277,20 +288,16 @@ __global__ void __launch_bounds__(32) qkv_fill_kernel(const __grid_constant__ Qk
 
   // ---- coefficients of this lane's pairs
   float coef[4][PP];
-  const void *weight = is_q ? p.q_weight : p.k_weight;
   float wa[PP], wb[PP];
 #pragma unroll
   for (int i = 0; i < PP; ++i) wa[i] = wb[i] = 1.f;
-  if (weight && w.mine)
-    R::split(__ldg(reinterpret_cast<const typename R::H *>(static_cast<const uint8_t *>(weight) + 2 * w.e0)),
-             __ldg(reinterpret_cast<const typename R::H *>(static_cast<const uint8_t *>(weight) + 2 * w.e1)), wa, wb);
+  if (weight && w.mine) R::split(weight_lo, weight_hi, wa, wb);
   const uint32_t half = p.rotary / 2;
 #pragma unroll
   for (int i = 0; i < PP; i += 4) {
     float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.axes) {
-      const int4 axis = w.turns ? __ldg(reinterpret_cast<const int4 *>(p.axes + w.pair + i)) : make_int4(0, 0, 0, 0);
-      const uint32_t of[4] = {(uint32_t)axis.x, (uint32_t)axis.y, (uint32_t)axis.z, (uint32_t)axis.w};
+      const uint32_t of[4] = {(uint32_t)axis[i / 4].x, (uint32_t)axis[i / 4].y, (uint32_t)axis[i / 4].z, (uint32_t)axis[i / 4].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t at = __shfl_sync(~0u, pos, min(of[k], p.n_axes - 1));
