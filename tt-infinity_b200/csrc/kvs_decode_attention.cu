@@ -16,14 +16,14 @@
 //     (16 tokens x 8 heads) and O^T = V^T P^T (16 elements x 8 heads), so a group of up to 8 heads
 //     fills the 8 columns and no instruction works on padding rows; groups up to 16 take two column
 //     tiles and larger ones several passes over the cache. (Memory is the bound: the tensor pipe is
-//     busy 8 % of the time for a bf16 cache, 16 % for e4m3.)
+//     busy 11 % of the time for a bf16 cache, 18 % for e4m3.)
 //   * Work is split by tokens, not by request: the batch's tiles, in units of a few tiles, form one
 //     sequence that is cut into equal runs, one per CTA, from lengths that only the device knows.
 //     A (request, head) that spans several CTAs leaves partial sums that a second small kernel
 //     joins, in the order of the sequence, so results do not depend on timing.
 // Device times, with the share of the measured copy rate: 48 contexts up to 16384 tokens, 8 KV heads of
-// 128, group 8, bf16: 233 us, 100 %; one of 131071: 89 us, 93 %; 64 up to 12001 from an e4m3 cache: 168 us,
-// 81 % (token-major pages of 16: a head's rows are 128 bytes in every 1024), 143 us, 95 % from head-major
+// 128, group 8, bf16: 234 us, 100 %; one of 131071: 88 us, 94 %; 64 up to 12001 from an e4m3 cache: 167 us,
+// 81 % (token-major pages of 16: a head's rows are 128 bytes in every 1024), 144 us, 94 % from head-major
 // pages.
 //
 // Scores, maxima, sums and accumulators are 32-bit. The probabilities are rounded to the cache's

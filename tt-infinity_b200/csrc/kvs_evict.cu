@@ -18,7 +18,7 @@
 // a second kernel moves the rows of one (request, head) by one CTA per 64-byte column of K or V, a
 // batch of ranks at a time: a kept token's rank is at most its position, so writing ranks [i, i + n)
 // only overwrites positions whose own rows have been read by then. 12 prompts of up to 32768 tokens, 8
-// heads, trimmed to 4096: 92 us, of which the rows' 370 MB take 57 us at the measured copy rate.
+// heads, trimmed to 4096: 88 us, of which the rows' 370 MB take 57 us, the measured copy rate.
 #include "kvs_paged_ops.cuh"
 
 #include <cooperative_groups.h>
@@ -489,9 +489,9 @@ __global__ void __launch_bounds__(kMoveThreads) move_in_place_kernel(const __gri
 cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   if (p.c.batch == 0) return cudaSuccess;
   const uint64_t cap = (uint64_t)p.c.max_blocks * p.c.block_size;
-  // CTAs per row: pieces of 1024 tokens while the GPU has room for more CTAs, of 8192 otherwise. (One
-  // row of 64-token pages per head, 16000 tokens, 8 heads: 19 us against 28 us with a CTA per row; 96
-  // rows of up to 32768 tokens: 92 us with four CTAs per row, 98 us with eight.)
+  // CTAs per row: pieces of 1024 tokens while SMs are left, of 8192 otherwise. 8 rows of 16000 tokens:
+  // 16 us against 38 us with a CTA per row; 64 rows of up to 8000: 36 us with four CTAs per row, 38 us
+  // with eight, 45 us with one; 96 rows of up to 32768: 88 us with four, 95 us with eight, 118 us with two.
   const uint64_t rows = (uint64_t)p.c.batch * p.c.n_heads;
   uint32_t ctas = 1;
   while (ctas < 8 && cap > 1024ull * ctas && (rows * ctas < 1ull * sms || cap > 8192ull * ctas)) ctas *= 2;

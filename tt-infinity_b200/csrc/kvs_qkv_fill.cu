@@ -16,7 +16,7 @@
 //     (a, b) -> (a A + b B, a C + b D) / sqrt(mean + eps)    A = wa cos, B = -wb sin, C = wa sin, D = wb cos
 // and the next rows are loaded while these are computed. Blocks of one warp: warps of a token differ in
 // length (queries, keys and values), and a block holds its registers until its last warp is done (72 us
-// against 60 us with blocks of two). 8192 tokens of 64 + 2 x 8 heads of 128: 57 us, 92 % of the measured
+// against 60 us with blocks of two). 8192 tokens of 64 + 2 x 8 heads of 128: 57 us, 93 % of the measured
 // copy rate.
 #include "kvs_paged_ops.cuh"
 
@@ -336,7 +336,7 @@ template <bool kBf, bool kInter, int PP, int kLanes>
 cudaError_t run(const QkvFillParams &p, cudaStream_t stream) {
   using R = Rows<kBf, kInter, PP, kLanes>;
   // Rows per warp: many share one lookup and one set of coefficients, as long as enough warps are left.
-  // 8192 tokens of 64 + 2 x 8 heads: 57 us with up to 64 rows per warp, 66 us with 16.
+  // 8192 tokens of 64 + 2 x 8 heads: 57 us with up to 64 rows per warp, 63 us with 16.
   const uint32_t steps = (p.q_heads + R::step - 1) / R::step;
   uint32_t per = 8;
   while (per > 1 && (uint64_t)p.tokens * ((steps + per - 1) / per) < 148 * 16) per /= 2;
