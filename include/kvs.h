@@ -337,7 +337,7 @@ int kvs_paged_fill_varlen_layers(uint32_t n_layers, const void *const *k_fills, 
  *
  * kvs_paged_cache describes one layer's cache: row (block, head, slot) of K is head_dim contiguous
  * elements at k + block * k_strides[0] + head * k_strides[1] + slot * k_strides[2] (bytes, multiples
- * of 16, as is the address; V likewise), which covers [num_blocks, heads, block_size, head_dim] and
+ * of 16, not negative; the address a multiple of 16; V likewise), which covers [num_blocks, heads, block_size, head_dim] and
  * vLLM's [num_blocks, block_size, heads, head_dim]. page_table: [batch][max_blocks] int32; entries
  * <= 0 hold nothing, entries >= num_blocks are out of range, and tokens in either take no part. An
  * e4m3 cache holds value / k_scale and value / v_scale, saturated; other types use scales of 1.
@@ -392,8 +392,8 @@ int kvs_qk_norm_rope_fill(const kvs_paged_cache *cache, const kvs_qkv_rows *rows
  * attends to its tokens [max(0, seq_lens[b] - window), seq_lens[b]) (window 0: all), seq_lens bounded
  * by max_blocks * block_size: out = sum softmax(scale * q . k) v. A row with no token gives zeros and
  * a log-sum-exp of -infinity. lse: optional [batch][q_heads] fp32, natural logarithm. weights_out
- * (optional, [batch][n_heads][w_len] fp32, strides in elements between requests and heads, may be
- * `weights`): weights_out[b][h][t] = weights[b][h][t] + the softmax weights of token t summed over the
+ * (optional, [batch][n_heads][w_len] fp32, strides in elements between requests and heads; `weights`
+ * itself, or apart from it): weights_out[b][h][t] = weights[b][h][t] + the softmax weights of token t summed over the
  * query heads of h, for t < seq_lens[b]; w_len must cover max_blocks * block_size. The order of every
  * sum is fixed by the lengths, so equal calls give equal bits. workspace: at least
  * kvs_decode_attention_workspace bytes, 256-byte aligned, its contents of no matter; concurrent
@@ -426,7 +426,7 @@ int kvs_paged_decode_attention(const kvs_paged_cache *cache, const kvs_decode_ro
  * of the call), or, where dst_table is null, of the request's own blocks, in place (then shared by no
  * other request). A slot without a valid block stores nothing and increments *out_of_range when
  * given. weights: [batch][n_heads][w_len] fp32 (strides in elements between requests and heads), w_len
- * covering max_blocks * block_size; weights_out (may be `weights`) receives the kept tokens' weights,
+ * covering max_blocks * block_size; weights_out (`weights` itself, or apart from it) receives the kept tokens' weights,
  * then zeros up to seq_lens[b]. cache->dtype gives the element size only: rows are moved as they are. */
 typedef struct {
   const int32_t *seq_lens, *dst_table;

@@ -7,18 +7,20 @@
 // Choosing: weights become 32-bit keys that sort as the weights do (0: no token, the largest: a
 // token that stays), and the keep-th largest key is found by its digits of 10, 8, 8 and 6 bits, most
 // significant first: a histogram of the keys that share the digits found so far, then the bin in
-// which the count from above reaches what is left. A cluster of up to 8 CTAs shares a row; the keys
-// stay in shared memory between the passes, so the weights are read from memory once, and the CTAs add
-// up one another's histograms there (digits of 12, 10 and 10 bits took longer: the exchange grows with
-// the bins). What bounds it is latency: four rounds of counting, exchange and scan, about 9 us for a
-// row of 4200 tokens. Chosen tokens are ranked by counting from the row's start, so the result does
-// not depend on timing.
+// which the count from above reaches what is left. Once few keys share the digits, they are ranked
+// against one another instead. A cluster of up to 8 CTAs shares a row; the keys stay in shared memory
+// between the passes, so the weights are read from memory once, and the CTAs add up one another's
+// histograms there (digits of 12, 10 and 10 bits took longer: the exchange grows with the bins). What
+// bounds it is latency for a few rows (counting, exchange, scan: about 9 us for 4200 tokens) and
+// instructions for many (28 us for 3.1 M weights). Chosen tokens are ranked by counting from the row's
+// start, so the result does not depend on timing.
 //
-// Moving: to fresh pages, each CTA moves the rows it chose of its tokens, in the same launch. In place,
-// a second kernel moves the rows of one (request, head) by one CTA per 64-byte column of K or V, a
-// batch of ranks at a time: a kept token's rank is at most its position, so writing ranks [i, i + n)
-// only overwrites positions whose own rows have been read by then. 12 prompts of up to 32768 tokens, 8
-// heads, trimmed to 4096: 88 us, of which the rows' 370 MB take 57 us, the measured copy rate.
+// Moving: a second kernel. To fresh pages, 64 ranks per CTA (12 prompts of up to 32768 tokens, 8 heads,
+// trimmed to 4096: 57 us of 88 us in all, the measured copy rate for 370 MB; moving in the first kernel,
+// by the CTA that chose the rows, took as long for many rows and longer for few). In place, one CTA per
+// 64-byte column of K or V of one (request, head), a batch of ranks at a time: a kept token's rank is at
+// most its position, so writing ranks [i, i + n) only overwrites positions whose own rows have been read
+// by then.
 #include "kvs_paged_ops.cuh"
 
 #include <cooperative_groups.h>

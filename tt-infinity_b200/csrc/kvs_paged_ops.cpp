@@ -70,7 +70,7 @@ struct Where {
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool strides16(const int64_t *s, int n) {
   for (int i = 0; i < n; ++i)
-    if (s[i] % 16) return false;
+    if (s[i] % 16 || s[i] < 0) return false;
   return true;
 }
 
@@ -90,7 +90,7 @@ int check_cache(const kvs_paged_cache *c, const char *op, kvs::PagedCache *out) 
         "%s: a page-table row must cover fewer than 2^31 tokens", op);
   CHECK(c->k && c->v && c->page_table, "%s: cache_k, cache_v or page_table must be on device!", op);
   CHECK(aligned16(c->k) && aligned16(c->v) && strides16(c->k_strides, 3) && strides16(c->v_strides, 3),
-        "%s: cache rows must start on 16-byte boundaries", op);
+        "%s: cache rows must start on 16-byte boundaries, with strides that are not negative", op);
   CHECK(std::isfinite(c->k_scale) && std::isfinite(c->v_scale) && c->k_scale > 0 && c->v_scale > 0,
         "%s: k_scale and v_scale must be positive and finite", op);
   CHECK(c->dtype == KVS_DTYPE_E4M3 || (c->k_scale == 1.f && c->v_scale == 1.f),
