@@ -356,11 +356,32 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   float *w_out = p.weights_out + (int64_t)b * p.wo_req + (int64_t)h * p.wo_head;
   const bool in_turn = w_out == w;  // then every weight of the row is read before one is written
   __syncthreads();
+  // the weights of ranks base, base + kSelThreads, ...: positions first, so that their loads overlap
+  constexpr uint32_t kRanks = 4;
+  auto weights_of = [&](uint32_t base, float (&x)[kRanks]) {
+    int32_t t[kRanks];
+#pragma unroll
+    for (uint32_t u = 0; u < kRanks; ++u) t[u] = base + u * kSelThreads < end ? kept[base + u * kSelThreads] : 0;
+#pragma unroll
+    for (uint32_t u = 0; u < kRanks; ++u) x[u] = base + u * kSelThreads < end ? w[t[u]] : 0.f;
+  };
   if (in_turn && cached)
-    for (uint32_t i = begin + tid; i < end; i += kSelThreads) s_keys[i - begin] = __float_as_uint(w[kept[i]]);
+    for (uint32_t i = begin + tid; i < end; i += kSelThreads * kRanks) {
+      float x[kRanks];
+      weights_of(i, x);
+#pragma unroll
+      for (uint32_t u = 0; u < kRanks; ++u)
+        if (i + u * kSelThreads < end) s_keys[i + u * kSelThreads - begin] = __float_as_uint(x[u]);
+    }
   cluster.sync();  // and no CTA leaves while another reads its counts
   if (!in_turn || cached) {
-    for (uint32_t i = begin + tid; i < end; i += kSelThreads) w_out[i] = in_turn ? __uint_as_float(s_keys[i - begin]) : __ldg(w + kept[i]);
+    for (uint32_t i = begin + tid; i < end; i += kSelThreads * kRanks) {
+      float x[kRanks];
+      if (!in_turn) weights_of(i, x);
+#pragma unroll
+      for (uint32_t u = 0; u < kRanks; ++u)
+        if (i + u * kSelThreads < end) w_out[i + u * kSelThreads] = in_turn ? __uint_as_float(s_keys[i + u * kSelThreads - begin]) : x[u];
+    }
     for (uint32_t i = want + rank * kSelThreads + tid; i < len; i += ctas * kSelThreads) w_out[i] = 0.f;
   }
 }
