@@ -139,6 +139,10 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   cg::cluster_group cluster = cg::this_cluster();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  auto sync_all = [&]() {  // a cluster's barrier costs several times a block's
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+  };
   const uint32_t row = blockIdx.x / ctas, b = row / p.c.n_heads, h = row % p.c.n_heads;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t len = length_of(p, b);
@@ -208,7 +212,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
       if (k.w) atomicAdd(&s_hist[k.w >> 22], 1u);
     }
   }
-  cluster.sync();
+  sync_all();
   Found f = find_bin<1024>(cluster, s_hist, p.keep, s_warp[0], s_out[0]);
   const uint32_t want = min(f.total, p.keep);
   // keys above `found` are chosen, and the first `left` equal to it; where all keys of a bin are
@@ -224,7 +228,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
       const uint4 k = quad_at(q);
       count(k.x), count(k.y), count(k.z), count(k.w);
     }
-    cluster.sync();
+    sync_all();
   };
   // Few keys share the digits found: every CTA collects them all and ranks each against the others.
   auto rank_few = [&](uint32_t low, uint32_t wanted, uint32_t total) {
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
       const uint4 k = quad_at(q);
       collect(k.x), collect(k.y), collect(k.z), collect(k.w);
     }
-    cluster.sync();
+    sync_all();
     const uint32_t theirs = lane < ctas ? *cluster.map_shared_rank(&s_few_count, lane) : 0;
     uint32_t before = 0, mine = 0;
     bool here = false;
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
       s_count[0] = of_above.y;
       s_count[1] = of_equal.y;
     }
-    cluster.sync();
+    sync_all();
     // lane r: the counts of CTA r, where it comes before this one
     const bool before = lane < rank;
     const uint32_t a = before ? *cluster.map_shared_rank(&s_count[0], lane) : 0, e = before ? *cluster.map_shared_rank(&s_count[1], lane) : 0;
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
       for (uint32_t u = 0; u < kRanks; ++u)
         if (i + u * kSelThreads < end) s_keys[i + u * kSelThreads - begin] = __float_as_uint(x[u]);
     }
-  cluster.sync();  // and no CTA leaves while another reads its counts
+  sync_all();  // and no CTA leaves while another reads its counts
   if (!in_turn || cached) {
     for (uint32_t i = begin + tid; i < end; i += kSelThreads * kRanks) {
       float x[kRanks];
