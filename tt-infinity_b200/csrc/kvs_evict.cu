@@ -16,7 +16,7 @@
 // start, so the result does not depend on timing.
 //
 // Moving: a second kernel. To fresh pages, 64 ranks per CTA (12 prompts of up to 32768 tokens, 8 heads,
-// trimmed to 4096: 57 us of 88 us in all, the measured copy rate for 370 MB; moving in the first kernel,
+// trimmed to 4096: 57 us of 87 us in all, the measured copy rate for 370 MB; moving in the first kernel,
 // by the CTA that chose the rows, took as long for many rows and longer for few). In place, one CTA per
 // 64-byte column of K or V of one (request, head), a batch of ranks at a time: a kept token's rank is at
 // most its position, so writing ranks [i, i + n) only overwrites positions whose own rows have been read
@@ -518,7 +518,7 @@ cudaError_t launch_evict(const EvictParams &p, int sms, cudaStream_t stream) {
   const uint64_t cap = (uint64_t)p.c.max_blocks * p.c.block_size;
   // CTAs per row: pieces of 1024 tokens while SMs are left, of 8192 otherwise. 8 rows of 16000 tokens:
   // 16 us against 38 us with a CTA per row; 64 rows of up to 8000: 36 us with four CTAs per row, 38 us
-  // with eight, 45 us with one; 96 rows of up to 32768: 88 us with four, 95 us with eight, 118 us with two.
+  // with eight, 45 us with one; 96 rows of up to 32768: 87 us with four, 95 us with eight, 118 us with two.
   const uint64_t rows = (uint64_t)p.c.batch * p.c.n_heads;
   uint32_t ctas = 1;
   while (ctas < 8 && cap > 1024ull * ctas && (rows * ctas < 1ull * sms || cap > 8192ull * ctas)) ctas *= 2;
