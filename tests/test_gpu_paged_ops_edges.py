@@ -1,0 +1,54 @@
+"""The operators on a paged cache at their edges: probabilities far below a row's largest, errors of a
+launch, tensors that autograd watches, and tables and sums that alias. 64-bit definitions and bounds are
+those of paged_ops_reference.py."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ops_reference as R
+from kvcache_manager import _native, ops
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def i32(x):
+    return torch.as_tensor(np.ascontiguousarray(x, dtype=np.int32)).cuda()
+
+
+@pytest.mark.parametrize("nats", [11, 15, 17, 19])
+@pytest.mark.parametrize("dtype,fp8", [(FP16, False), (FP16, True), (BF16, True)])
+@pytest.mark.parametrize("batch,length", [(40, 512), (1, 4096)])
+def test_attention_behind_a_sink(batch, length, dtype, fp8, nats):
+    """The first token's score is `nats` above the others' and its value is zero, so that the others'
+    probabilities, of e^-nats each, make up the whole output. The 512-token rows are a CTA each, 128 tokens
+    sharing the sink's warp; the long row is split."""
+    g, page, dim, group = gen(nats), 16, 64, 2
+    pages = length // page
+    table = (torch.randperm(batch * pages, generator=g) + 1).reshape(batch, pages).numpy().astype(np.int32)
+    shape = (batch * pages + 1, 1, page, dim)
+    k = 0.05 * torch.randn(shape, generator=g)
+    v = (300 + 50 * torch.randn(shape, generator=g)).clamp(150, 440)
+    k[table[:, 0], 0, 0] = nats * dim**-0.5
+    v[table[:, 0], 0, 0] = 0
+    q = (1 + 0.1 * torch.randn((batch, group, dim), generator=g)).to(dtype)
+    ks, vs = (0.0625, 1.0) if fp8 else (1.0, 1.0)
+    k, v = ((k / ks).to(E4M3), v.to(E4M3)) if fp8 else (k.to(dtype), v.to(dtype))
+    lens = [length] * batch
+    out, _, _, b_out, _, _ = R.attend(R.f64(q), R.f64(k), R.f64(v), table, lens, dim**-0.5, 0, ks, vs, dtype, fp8)
+    # The bound allows each fp16 probability half of the smallest fp16 step, 2^-25, relative to the largest
+    # one. Held 2^15 times larger (at most 2^15 < 65504), it is off by half a step of itself, which the bound
+    # holds already, or by 2^-25 2^-15 of the largest.
+    top = np.abs(R.f64(v)).max() * vs
+    b_out = b_out - length * 2.0**-25 * top + length * 2.0**-40 * top
+    assert (b_out < 0.05 * np.abs(out)).all()  # what the bound leaves is small beside the output
+    got = R.f64(ops.paged_decode_attention(q.cuda(), k.cuda(), v.cuda(), i32(table), i32(lens), k_scale=ks, v_scale=vs))
+    assert (np.abs(got - out) <= b_out).all(), (np.abs(got - out) / np.abs(out)).max()
