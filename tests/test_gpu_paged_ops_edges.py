@@ -52,3 +52,53 @@ def test_attention_behind_a_sink(batch, length, dtype, fp8, nats):
     assert (b_out < 0.05 * np.abs(out)).all()  # what the bound leaves is small beside the output
     got = R.f64(ops.paged_decode_attention(q.cuda(), k.cuda(), v.cuda(), i32(table), i32(lens), k_scale=ks, v_scale=vs))
     assert (np.abs(got - out) <= b_out).all(), (np.abs(got - out) / np.abs(out)).max()
+
+
+def decode_args(q_heads=4, dim=64):
+    """Arguments of the three operators on one small cache (2 requests, 2 KV heads, pages of 16)."""
+    g = gen(1)
+    randn = lambda *s: torch.randn(s, generator=g).to(BF16).cuda()
+    ck, cv = randn(8, 2, 16, dim), randn(8, 2, 16, dim)
+    table = i32([[1, 2], [3, 4]])
+    angle = torch.rand((64, dim // 2), generator=g)
+    fill = dict(q=randn(2, q_heads, dim), k=randn(2, 2, dim), v=randn(2, 2, dim),
+                cos_sin=torch.cat([angle.cos(), angle.sin()], 1).cuda(), cu_seqlens=i32([0, 1, 2]), page_table=table,
+                start_positions=i32([28, 17]), cache_k=ck, cache_v=cv)
+    attend = dict(q=randn(2, q_heads, dim), cache_k=ck, cache_v=cv, page_table=table, seq_lens=i32([29, 18]),
+                  weights=torch.rand((2, 2, 32), generator=g).cuda())
+    evict = dict(cache_k=ck, cache_v=cv, page_table=table, seq_lens=i32([29, 18]), weights=torch.rand((2, 2, 32), generator=g).cuda(),
+                 keep=10, dst_page_table=i32([[5], [6]]))
+    return fill, attend, evict
+
+
+@pytest.mark.parametrize("which", ["fill", "attend", "evict"])
+def test_failed_launch_is_reported_and_not_repeated(which, monkeypatch):
+    """An error that is no refusal of the arguments ends the call: part of its work may have been
+    enqueued. Entry points that only return such an error stand in for the library's."""
+    opcall = _native.load_opcall()
+    assert opcall
+    lib, calls = _native.load(), []
+    args = dict(zip(("fill", "attend", "evict"), decode_args()))[which]
+    operator = {"fill": ops.qk_norm_rope_fill, "attend": ops.paged_decode_attention, "evict": ops.evict_paged_kv}[which]
+    addr = lambda fn: C.cast(fn, C.c_void_p).value
+    real = [addr(f) for f in (lib.kvs_qk_norm_rope_fill, lib.kvs_decode_attention_workspace, lib.kvs_paged_decode_attention, lib.kvs_evict_paged)]
+
+    @C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_void_p, C.c_void_p)
+    def failing(cache, rows, stream):
+        calls.append("compiled")
+        return _native.E_CUDA
+
+    class Repeats:  # what the ctypes path would call
+        def __getattr__(self, name):
+            if name in ("kvs_qk_norm_rope_fill", "kvs_paged_decode_attention", "kvs_evict_paged"):
+                return lambda *a: calls.append("repeated") or _native.OK
+            return getattr(lib, name)
+
+    monkeypatch.setattr(ops, "load", lambda: Repeats())
+    opcall.bind(addr(failing), real[1], addr(failing), addr(failing))
+    try:
+        with pytest.raises(_native.KvsError) as e:
+            operator(**args)
+    finally:
+        opcall.bind(*real)
+    assert calls == ["compiled"] and e.value.code == _native.E_CUDA

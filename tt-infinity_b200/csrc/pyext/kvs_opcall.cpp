@@ -6,9 +6,11 @@
  * the outputs and calls the functions of libkvs_b200.so through pointers that the package hands over
  * once (bind), so both bindings use the one loaded library.
  *
- * A call returns NotImplemented for whatever it does not take (a failed check, a tensor subclass, an
- * error from the library); the caller then takes its ctypes path, which repeats the checks and raises
- * the error with its message. */
+ * A call returns NotImplemented for whatever it does not take (a failed check, here or in the library, or
+ * a tensor subclass); the caller then takes its ctypes path, which repeats the checks and raises the error
+ * with its message. Any other error of the library comes back as its status, an int, for the caller to
+ * raise: work may have been enqueued, and repeating it (rows turned in place, weights compacted in place)
+ * would change what it reads. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -132,21 +134,27 @@ bool sums_fit(const at::Tensor &t, int64_t batch, int64_t heads, int64_t cover) 
 }
 
 PyObject *not_taken() { Py_RETURN_NOTIMPLEMENTED; }
+// KVS_E_INVAL is a check's, before anything is enqueued
+PyObject *failed(int rc) { return rc == KVS_E_INVAL ? not_taken() : PyLong_FromLong(rc); }
 
-// A call whose C++ exceptions end here: the ctypes path says what was wrong.
-template <PyObject *(*call)(PyObject *const *)>
+// A call whose C++ exceptions end here: before the library was called the ctypes path says what was wrong,
+// after that nothing is repeated.
+template <PyObject *(*call)(PyObject *const *, bool &)>
 PyObject *guarded(PyObject *const *args) {
+  bool called = false;
   try {
-    return call(args);
-  } catch (const std::exception &) {
+    return call(args, called);
+  } catch (const std::exception &e) {
     if (PyErr_Occurred()) PyErr_Clear();
-    return not_taken();
+    if (!called) return not_taken();
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
   }
 }
 
 // fill(q, k, v, cos_sin, cu_seqlens, page_table, start_positions, cache_k, cache_v, q_weight, k_weight,
 //      eps, positions, axes, interleaved, k_scale, v_scale, q_out, out_of_range) -> q_out
-PyObject *take_fill(PyObject *const *args) {
+PyObject *take_fill(PyObject *const *args, bool &called) {
   Call c{args};
   kvs_paged_cache cache;
   if (!cache_of(c, 7, 5, 15, &cache)) return not_taken();
@@ -195,10 +203,11 @@ PyObject *take_fill(PyObject *const *args) {
   if (!c.ok) return not_taken();
   void *stream = c.stream();
   int rc;
+  called = true;
   Py_BEGIN_ALLOW_THREADS
   rc = g_fill(&cache, &r, stream);
   Py_END_ALLOW_THREADS
-  if (rc != KVS_OK) return not_taken();
+  if (rc != KVS_OK) return failed(rc);
   if (out) {
     Py_INCREF(args[17]);
     return args[17];
@@ -211,7 +220,7 @@ PyObject *fill(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // attend(q, cache_k, cache_v, page_table, seq_lens, scale, window, k_scale, v_scale, out, return_lse, weights,
 //        weights_out) -> out or (out, lse)
-PyObject *take_attend(PyObject *const *args) {
+PyObject *take_attend(PyObject *const *args, bool &called) {
   Call c{args};
   kvs_paged_cache cache;
   if (!cache_of(c, 1, 3, 7, &cache)) return not_taken();
@@ -245,15 +254,17 @@ PyObject *take_attend(PyObject *const *args) {
   }
   r.q_heads = heads, r.window = window, r.dtype = code_of(q->scalar_type());
   r.scale = args[5] == Py_None ? (float)(1.0 / std::sqrt((double)dim)) : (float)c.number(5);
-  if (!c.ok || g_workspace(&cache, &r, c.device.index(), &r.workspace_bytes) != KVS_OK) return not_taken();
+  if (!c.ok) return not_taken();
+  if (const int bad = g_workspace(&cache, &r, c.device.index(), &r.workspace_bytes)) return failed(bad);
   const at::Tensor workspace = at::empty({(int64_t)r.workspace_bytes}, q->options().dtype(at::kByte));
   r.workspace = workspace.data_ptr();
   void *stream = c.stream();
   int rc;
+  called = true;
   Py_BEGIN_ALLOW_THREADS
   rc = g_attend(&cache, &r, stream);
   Py_END_ALLOW_THREADS
-  if (rc != KVS_OK) return not_taken();
+  if (rc != KVS_OK) return failed(rc);
   PyObject *result;
   if (out) {
     Py_INCREF(args[9]);
@@ -274,7 +285,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // evict(cache_k, cache_v, page_table, seq_lens, weights, keep, first, recent, dst_page_table, weights_out,
 //       out_of_range) -> (kept, new_lens)
-PyObject *take_evict(PyObject *const *args) {
+PyObject *take_evict(PyObject *const *args, bool &called) {
   Call c{args};
   kvs_paged_cache cache;
   if (!cache_of(c, 0, 2, -1, &cache)) return not_taken();
@@ -304,10 +315,11 @@ PyObject *take_evict(PyObject *const *args) {
   r.keep = keep, r.first = first, r.recent = recent;
   void *stream = c.stream();
   int rc;
+  called = true;
   Py_BEGIN_ALLOW_THREADS
   rc = g_evict(&cache, &r, stream);
   Py_END_ALLOW_THREADS
-  if (rc != KVS_OK) return not_taken();
+  if (rc != KVS_OK) return failed(rc);
   PyObject *a = THPVariable_Wrap(kept), *b = a ? THPVariable_Wrap(fresh) : nullptr;
   PyObject *both = b ? PyTuple_Pack(2, a, b) : nullptr;
   Py_XDECREF(a);

@@ -310,6 +310,13 @@ def _ptr(t: Any):
 _S2 = C.c_int64 * 2
 
 
+def _taken(done: Any) -> Any:
+    """What the compiled entry returned; an error of a launch, which is not repeated, is its status."""
+    if isinstance(done, int):
+        check(done)
+    return done
+
+
 def qk_norm_rope_fill(q: Any, k: Any, v: Any, cos_sin: Any, cu_seqlens: Any, page_table: Any, start_positions: Any,
                       cache_k: Any, cache_v: Any, *, q_weight: Any = None, k_weight: Any = None, eps: float = 1e-6,
                       positions: Any = None, axes: Any = None, interleaved: bool = False, k_scale: float = 1.0,
@@ -340,7 +347,7 @@ def qk_norm_rope_fill(q: Any, k: Any, v: Any, cos_sin: Any, cu_seqlens: Any, pag
         done = fast.fill(q, k, v, cos_sin, cu_seqlens, page_table, start_positions, cache_k, cache_v, q_weight, k_weight,
                          eps, positions, axes, interleaved, k_scale, v_scale, q_out, out_of_range)
         if done is not NotImplemented:
-            return done, cache_k, cache_v
+            return _taken(done), cache_k, cache_v
     torch = _torch()
     cache = _paged_cache(cache_k, cache_v, page_table, k_scale, v_scale)
     dev = cache_k.device
@@ -424,7 +431,7 @@ def paged_decode_attention(q: Any, cache_k: Any, cache_v: Any, page_table: Any, 
         done = fast.attend(q, cache_k, cache_v, page_table, seq_lens, scale, window, k_scale, v_scale, out, return_lse,
                            weights, weights_out)
         if done is not NotImplemented:
-            return done
+            return _taken(done)
     torch = _torch()
     cache = _paged_cache(cache_k, cache_v, page_table, k_scale, v_scale)
     dev = cache_k.device
@@ -497,7 +504,7 @@ def evict_paged_kv(cache_k: Any, cache_v: Any, page_table: Any, seq_lens: Any, w
         done = fast.evict(cache_k, cache_v, page_table, seq_lens, weights, keep, first, recent, dst_page_table,
                           weights_out, out_of_range)
         if done is not NotImplemented:
-            return done
+            return _taken(done)
     torch = _torch()
     cache = _paged_cache(cache_k, cache_v, page_table, 1.0, 1.0)
     dev = cache_k.device
