@@ -102,3 +102,43 @@ def test_failed_launch_is_reported_and_not_repeated(which, monkeypatch):
     finally:
         opcall.bind(*real)
     assert calls == ["compiled"] and e.value.code == _native.E_CUDA
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_error_of_an_earlier_call_is_not_taken_for_the_launches(compiled, monkeypatch):
+    """A call that failed and said so (a device that is not there) leaves nothing behind: the next ones
+    run once and report success."""
+    if not compiled:
+        monkeypatch.setattr(_native, "opcall", False)
+    lib = _native.load()
+
+    def earlier_failure():
+        cache = _native.PagedCache(1 << 20, 1 << 20, (C.c_int64 * 3)(4096, 2048, 128), (C.c_int64 * 3)(4096, 2048, 128), 1 << 20, 4, 2, 16, 64,
+                                   2, 2, _native.DTYPE_BF16, 1.0, 1.0)
+        rows = _native.DecodeRows(q_heads=4)
+        assert lib.kvs_decode_attention_workspace(C.byref(cache), C.byref(rows), 999, C.byref(C.c_uint64())) == _native.E_CUDA
+
+    fill, attend, _ = decode_args()
+    want, _, _ = ops.qk_norm_rope_fill(**fill)
+    out = ops.paged_decode_attention(**dict(attend, weights=None))
+    count = torch.zeros(1, dtype=torch.int32, device="cuda")
+    fill["page_table"] = i32([[1, 99], [3, 4]])  # a token in a page that is not there is counted once
+    earlier_failure()
+    got, _, _ = ops.qk_norm_rope_fill(**fill, q_out=fill["q"], out_of_range=count)  # in place: turned once
+    assert torch.equal(got, want) and int(count) == 1
+    earlier_failure()
+    assert torch.equal(ops.paged_decode_attention(**dict(attend, weights=None)), out)
+
+
+def test_failed_server_leaves_no_error_behind():
+    """A server whose slab no GPU holds is refused; the next launch of the library is not blamed for it."""
+    lib = _native.load()
+    config = _native.ServerConfig()
+    assert lib.kvs_server_config_default(C.byref(config)) == _native.OK
+    config.heap_bytes, config.unit_bytes, config.max_keys, config.host_pool_bytes = 1 << 46, 1 << 24, 64, 0
+    server = C.c_void_p()
+    assert lib.kvs_server_create(C.byref(config), C.byref(server)) == _native.E_NOSPACE
+    k = torch.ones((1, 2, 4, 64), dtype=BF16, device="cuda")
+    ck, cv = (torch.zeros((3, 2, 16, 64), dtype=BF16, device="cuda") for _ in range(2))
+    ops.paged_fill_cache_varlen(k, k, i32([0, 4]), i32([[2]]), i32([3]), ck, cv)
+    assert (ck[2, :, 3:7] == 1).all() and ck.sum() == 2 * 4 * 64

@@ -1002,9 +1002,9 @@ __global__ void __launch_bounds__(256, 3) finish_kernel(const __grid_constant__ 
   else add_weights<NT>(p, blockIdx.x - p.join_blocks);
 }
 
-template <class K, class... Args>
-cudaError_t launch_after(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
-  // starts while the kernel before it drains; it waits for that kernel's results itself
+// `after`: starts while the kernel before it drains, and waits for that kernel's results itself.
+template <class K>
+cudaError_t launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const KernelParams &kp, bool after) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -1014,9 +1014,10 @@ cudaError_t launch_after(K kernel, dim3 grid, dim3 block, size_t smem, cudaStrea
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
-  count_launch();
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
+  cfg.numAttrs = after;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, kp);  // this launch's own error, no earlier call's
+  if (e == cudaSuccess) count_launch();
+  return e;
 }
 
 template <int kKind, int DP, int NT>
@@ -1033,9 +1034,7 @@ cudaError_t run(const KernelParams &kp, const Plan &plan, int sms, cudaStream_t 
     if (e != cudaSuccess) return e;
     if (dev < 64) ready.fetch_or(bit, std::memory_order_release);
   }
-  kernel<<<plan.grid, kThreads, C::smem, stream>>>(kp);
-  count_launch();
-  e = cudaGetLastError();
+  e = launch(kernel, dim3(plan.grid), dim3(kThreads), C::smem, stream, kp, false);
   if (e != cudaSuccess) return e;
   KernelParams fp = kp;
   // Fragments a joining block takes: up to eight, a warp each, which suits requests of a few parts; where
@@ -1057,7 +1056,7 @@ cudaError_t run(const KernelParams &kp, const Plan &plan, int sms, cudaStream_t 
   }
   if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidValue;
   if (blocks)
-    e = launch_after(finish_kernel<DP, NT, kKind == kKindE4m3>, dim3((unsigned)blocks), dim3(256), kp.logits ? 4ull * (kp.group + 3) : 0, stream, fp);
+    e = launch(finish_kernel<DP, NT, kKind == kKindE4m3>, dim3((unsigned)blocks), dim3(256), kp.logits ? 4ull * (kp.group + 3) : 0, stream, fp, true);
   return e;
 }
 

@@ -68,6 +68,7 @@ int fail(int code, const char *fmt, ...) {
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
   kvs::set_last_error(buf);  // reported by kvs_last_error()
+  if (code == KVS_E_CUDA) cudaGetLastError();  // and by no later launch
   return code;
 }
 

@@ -20,6 +20,7 @@ int fail(int code, const char *fmt, ...) {
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
   kvs::set_last_error(buf);
+  if (code == KVS_E_CUDA) cudaGetLastError();  // reported here, and by no later launch
   return code;
 }
 

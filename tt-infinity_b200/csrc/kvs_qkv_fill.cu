@@ -343,9 +343,14 @@ cudaError_t run(const QkvFillParams &p, cudaStream_t stream) {
   const uint32_t q_parts = (steps + per - 1) / per, kv_parts = (p.c.n_heads + per * R::step - 1) / (per * R::step);
   const dim3 grid(p.tokens, q_parts + kv_parts);
   if (grid.y > 65535) return cudaErrorInvalidValue;
-  qkv_fill_kernel<kBf, kInter, PP, kLanes><<<grid, 32, 0, stream>>>(p, q_parts, per * R::step);
-  count_launch();
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(32);
+  cfg.stream = stream;
+  // this launch's own error, no earlier call's
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, qkv_fill_kernel<kBf, kInter, PP, kLanes>, p, q_parts, per * R::step);
+  if (e == cudaSuccess) count_launch();
+  return e;
 }
 
 template <bool kBf, bool kInter>

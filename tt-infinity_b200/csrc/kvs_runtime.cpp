@@ -54,6 +54,7 @@ int set_err(int code, const char *fmt, ...) {
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
   g_err = buf;
+  if (code == KVS_E_CUDA || code == KVS_E_NOSPACE) cudaGetLastError();  // reported here, and by no later launch
   return code;
 }
 
