@@ -142,3 +142,18 @@ def test_failed_server_leaves_no_error_behind():
     ck, cv = (torch.zeros((3, 2, 16, 64), dtype=BF16, device="cuda") for _ in range(2))
     ops.paged_fill_cache_varlen(k, k, i32([0, 4]), i32([[2]]), i32([3]), ck, cv)
     assert (ck[2, :, 3:7] == 1).all() and ck.sum() == 2 * 4 * 64
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_tangents_are_refused(compiled, monkeypatch):
+    if not compiled:
+        monkeypatch.setattr(_native, "opcall", False)
+    fill, attend, evict = decode_args()
+    for operator, args, names in ((ops.qk_norm_rope_fill, fill, ("q", "k", "v", "cos_sin", "cache_k")),
+                                  (ops.paged_decode_attention, attend, ("q", "cache_v", "weights")), (ops.evict_paged_kv, evict, ("weights",))):
+        for name in names:
+            with torch.autograd.forward_ad.dual_level():
+                dual = torch.autograd.forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+                with pytest.raises(RuntimeError, match=f"{name} carries a tangent"):
+                    operator(**dict(args, **{name: dual}))
+        operator(**args)

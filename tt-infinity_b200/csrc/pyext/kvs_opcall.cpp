@@ -30,7 +30,7 @@ int (*g_workspace)(const kvs_paged_cache *, const kvs_decode_rows *, int32_t, ui
 int (*g_attend)(const kvs_paged_cache *, const kvs_decode_rows *, void *);
 int (*g_evict)(const kvs_paged_cache *, const kvs_evict_rows *, void *);
 
-// The arguments of one call: tensors on one GPU, of which none needs a gradient.
+// The arguments of one call: tensors on one GPU, of which none needs a gradient or carries a tangent.
 struct Call {
   PyObject *const *args;
   c10::Device device{c10::kCPU};
@@ -42,7 +42,8 @@ struct Call {
     if (o == Py_None && optional) return nullptr;
     if (!THPVariable_CheckExact(o)) return fail();
     const at::Tensor &t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.dim() != dims || t.layout() != c10::kStrided || (grad && t.requires_grad())) return fail();
+    if (!t.is_cuda() || t.dim() != dims || t.layout() != c10::kStrided || (grad && t.requires_grad()) || t._fw_grad(0).defined())
+      return fail();
     if (device.is_cpu()) device = t.device();
     if (t.device() != device) return fail();
     return &t;

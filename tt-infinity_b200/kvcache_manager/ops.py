@@ -234,7 +234,8 @@ def _dtype_code(dtype: Any) -> int:
 
 
 def _on(device: Any, **tensors: Any) -> None:
-    """Every tensor given (None: not given) is a CUDA tensor on `device` that needs no gradient."""
+    """Every tensor given (None: not given) is a CUDA tensor on `device` that needs no gradient and
+    carries no tangent."""
     torch = _torch()
     for name, t in tensors.items():
         if t is None:
@@ -245,6 +246,8 @@ def _on(device: Any, **tensors: Any) -> None:
             raise RuntimeError("All tensors must be on the same device!")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires grad, and the operators on a paged cache have no backward pass")
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} carries a tangent, and the operators on a paged cache have no derivatives")
 
 
 def _int32(ndim: int, **tensors: Any) -> None:
