@@ -157,3 +157,44 @@ def test_tangents_are_refused(compiled, monkeypatch):
                 with pytest.raises(RuntimeError, match=f"{name} carries a tangent"):
                     operator(**dict(args, **{name: dual}))
         operator(**args)
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_written_tensors_count_as_changed(compiled, monkeypatch):
+    """autograd refuses a backward pass through a tensor that a call has overwritten since."""
+    if not compiled:
+        monkeypatch.setattr(_native, "opcall", False)
+    fill, attend, evict = decode_args()
+    count = lambda: torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.zeros_like(attend["q"])
+    sums = torch.zeros_like(attend["weights"])
+    calls = [(ops.qk_norm_rope_fill, dict(fill, q_out=fill["q"], out_of_range=count()), ("q", "cache_k", "cache_v", "out_of_range"), ("k", "cos_sin")),
+             (ops.paged_decode_attention, dict(attend, out=out), ("out", "weights"), ("q", "cache_k", "cache_v")),
+             (ops.paged_decode_attention, dict(attend, weights_out=sums), ("weights_out",), ("weights",)),
+             (ops.evict_paged_kv, dict(evict, out_of_range=count()), ("cache_k", "cache_v", "weights", "out_of_range"), ("seq_lens", "dst_page_table")),
+             (ops.evict_paged_kv, dict(evict, weights_out=sums), ("weights_out",), ("weights",))]
+    for operator, args, written, kept in calls:
+        before = {name: args[name]._version for name in written + kept}
+        operator(**args)
+        assert all(args[name]._version > before[name] for name in written), (operator, written)
+        assert all(args[name]._version == before[name] for name in kept), (operator, kept)
+    x = torch.ones(64, device="cuda", dtype=BF16, requires_grad=True)
+    fill, _, _ = decode_args()
+    y = (fill["q"] * x).sum()
+    ops.qk_norm_rope_fill(**fill, q_out=fill["q"])
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.backward()
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_inference_tensors_are_written(compiled, monkeypatch):
+    if not compiled:
+        monkeypatch.setattr(_native, "opcall", False)
+    with torch.inference_mode():
+        fill, attend, evict = decode_args()
+    want, _, _ = ops.qk_norm_rope_fill(**fill)
+    with torch.inference_mode():
+        for operator, args in ((ops.paged_decode_attention, attend), (ops.evict_paged_kv, evict)):
+            operator(**args)
+    got, _, _ = ops.qk_norm_rope_fill(**fill, q_out=fill["q"])
+    assert torch.equal(got, want)

@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <initializer_list>
 
 #include "kvs.h"
 
@@ -134,6 +135,13 @@ bool sums_fit(const at::Tensor &t, int64_t batch, int64_t heads, int64_t cover) 
          t.size(2) <= INT32_MAX;
 }
 
+// What a call has written counts as changed, so that autograd refuses a backward pass that saved it
+// (tensors made in inference mode keep no count).
+void changed(std::initializer_list<const at::Tensor *> written) {
+  for (const at::Tensor *t : written)
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 PyObject *not_taken() { Py_RETURN_NOTIMPLEMENTED; }
 // KVS_E_INVAL is a check's, before anything is enqueued
 PyObject *failed(int rc) { return rc == KVS_E_INVAL ? not_taken() : PyLong_FromLong(rc); }
@@ -209,6 +217,7 @@ PyObject *take_fill(PyObject *const *args, bool &called) {
   rc = g_fill(&cache, &r, stream);
   Py_END_ALLOW_THREADS
   if (rc != KVS_OK) return failed(rc);
+  changed({&THPVariable_Unpack(args[7]), &THPVariable_Unpack(args[8]), out, count});
   if (out) {
     Py_INCREF(args[17]);
     return args[17];
@@ -266,6 +275,7 @@ PyObject *take_attend(PyObject *const *args, bool &called) {
   rc = g_attend(&cache, &r, stream);
   Py_END_ALLOW_THREADS
   if (rc != KVS_OK) return failed(rc);
+  changed({out, wo});
   PyObject *result;
   if (out) {
     Py_INCREF(args[9]);
@@ -321,6 +331,7 @@ PyObject *take_evict(PyObject *const *args, bool &called) {
   rc = g_evict(&cache, &r, stream);
   Py_END_ALLOW_THREADS
   if (rc != KVS_OK) return failed(rc);
+  changed({&THPVariable_Unpack(args[0]), &THPVariable_Unpack(args[1]), wo, count});
   PyObject *a = THPVariable_Wrap(kept), *b = a ? THPVariable_Wrap(fresh) : nullptr;
   PyObject *both = b ? PyTuple_Pack(2, a, b) : nullptr;
   Py_XDECREF(a);

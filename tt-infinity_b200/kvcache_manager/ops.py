@@ -306,6 +306,14 @@ def _check_counter(t: Any) -> None:
         raise RuntimeError("out_of_range must be an int32 tensor of one element")
 
 
+def _changed(*written: Any) -> None:
+    """What a call has written counts as changed, so that autograd refuses a backward pass that saved
+    it (tensors made in inference mode keep no count)."""
+    for t in written:
+        if t is not None and not t.is_inference():
+            _torch().autograd.graph.increment_version(t)
+
+
 def _ptr(t: Any):
     return None if t is None else t.data_ptr()
 
@@ -399,6 +407,7 @@ def qk_norm_rope_fill(q: Any, k: Any, v: Any, cos_sin: Any, cu_seqlens: Any, pag
         start_positions.data_ptr(), _ptr(positions), _ptr(axes), _ptr(q_weight), _ptr(k_weight), _ptr(out_of_range),
         tokens, q_heads, cos_sin.shape[1], cos_sin.shape[0], n_axes, _dtype_code(q.dtype), eps, interleaved, zero_rest)
     check(load().kvs_qk_norm_rope_fill(C.byref(cache), C.byref(rows), _stream(dev)))
+    _changed(cache_k, cache_v, None if zero_rest else q_out, out_of_range)
     return q_out, cache_k, cache_v
 
 
@@ -448,6 +457,7 @@ def paged_decode_attention(q: Any, cache_k: Any, cache_v: Any, page_table: Any, 
         raise RuntimeError(f"seq_lens size ({seq_lens.shape[0]}) must match batch_size ({batch})")
     if window is not None and not 0 < window < 1 << 31:
         raise RuntimeError("window must be 1 to 2^31 - 1 tokens")
+    given = out
     if out is None:
         out = torch.empty((batch, q_heads, dim), dtype=q.dtype, device=dev)
     else:
@@ -480,6 +490,7 @@ def paged_decode_attention(q: Any, cache_k: Any, cache_v: Any, page_table: Any, 
     workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
     rows.workspace, rows.workspace_bytes = workspace.data_ptr(), need.value
     check(lib.kvs_paged_decode_attention(C.byref(cache), C.byref(rows), _stream(dev)))
+    _changed(given, weights_out)
     return (out, lse) if return_lse else out
 
 
@@ -537,4 +548,5 @@ def evict_paged_kv(cache_k: Any, cache_v: Any, page_table: Any, seq_lens: Any, w
         new_lens.data_ptr(), _ptr(out_of_range), 0 if in_place else dst_page_table.shape[1], weights.shape[2],
         weights_out.shape[2], keep, first, recent)
     check(load().kvs_evict_paged(C.byref(cache), C.byref(rows), _stream(dev)))
+    _changed(cache_k, cache_v, weights_out, out_of_range)
     return kept, new_lens
