@@ -340,7 +340,8 @@ int kvs_paged_fill_varlen_layers(uint32_t n_layers, const void *const *k_fills, 
  * of 16, not negative; the address a multiple of 16; V likewise), which covers [num_blocks, heads, block_size, head_dim] and
  * vLLM's [num_blocks, block_size, heads, head_dim]. page_table: [batch][max_blocks] int32; entries
  * <= 0 hold nothing, entries >= num_blocks are out of range, and tokens in either take no part. An
- * e4m3 cache holds value / k_scale and value / v_scale, saturated; other types use scales of 1.
+ * e4m3 cache holds value / k_scale and value / v_scale, saturated; other types use scales of 1. A scale
+ * is positive and finite, and so is its reciprocal.
  * head_dim: a multiple of 8 (16 for e4m3) up to 256. Rows behind a request's length, and all that a
  * masked slot holds, are not read. All arrays are device memory of one GPU; calls are asynchronous
  * on `stream`, make no allocation and keep no state, so they can be captured into CUDA graphs. */

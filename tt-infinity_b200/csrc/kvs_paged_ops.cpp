@@ -94,6 +94,8 @@ int check_cache(const kvs_paged_cache *c, const char *op, kvs::PagedCache *out) 
         "%s: cache rows must start on 16-byte boundaries, with strides that are not negative", op);
   CHECK(std::isfinite(c->k_scale) && std::isfinite(c->v_scale) && c->k_scale > 0 && c->v_scale > 0,
         "%s: k_scale and v_scale must be positive and finite", op);
+  CHECK(std::isfinite(1.f / c->k_scale) && std::isfinite(1.f / c->v_scale),
+        "%s: k_scale and v_scale must have a finite reciprocal", op);
   CHECK(c->dtype == KVS_DTYPE_E4M3 || (c->k_scale == 1.f && c->v_scale == 1.f),
         "%s: k_scale and v_scale belong to an e4m3 cache", op);
   *out = kvs::PagedCache{static_cast<uint8_t *>(c->k), static_cast<uint8_t *>(c->v),
