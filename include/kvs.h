@@ -424,8 +424,8 @@ int kvs_paged_decode_attention(const kvs_paged_cache *cache, const kvs_decode_ro
  * in all (first + recent <= keep). kept: [batch][n_heads][keep] int32, the kept positions in order,
  * then -1; new_lens: [batch] int32, min(keep, tokens). Kept rows of K and V move to slots 0, 1, ... of
  * dst_table ([batch][dst_blocks] int32, covering keep slots; its blocks must be in no other table row
- * of the call), or, where dst_table is null, of the request's own blocks, in place (then shared by no
- * other request). A slot without a valid block stores nothing and increments *out_of_range when
+ * of the call), or, where dst_table is null or the page table itself, of the request's own blocks, in
+ * place (then shared by no other request). A slot without a valid block stores nothing and increments *out_of_range when
  * given. weights: [batch][n_heads][w_len] fp32 (strides in elements between requests and heads), w_len
  * covering max_blocks * block_size; weights_out (`weights` itself, or apart from it) receives the kept tokens' weights,
  * then zeros up to seq_lens[b]. cache->dtype gives the element size only: rows are moved as they are. */

@@ -198,3 +198,20 @@ def test_inference_tensors_are_written(compiled, monkeypatch):
             operator(**args)
     got, _, _ = ops.qk_norm_rope_fill(**fill, q_out=fill["q"])
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_evict_destination_that_is_the_front_of_the_table(compiled, monkeypatch):
+    if not compiled:
+        monkeypatch.setattr(_native, "opcall", False)
+    g = gen(5)
+    ck, cv = (torch.randn((10, 2, 16, 64), generator=g).to(BF16).cuda() for _ in range(2))
+    w = torch.rand((1, 2, 128), generator=g).cuda()
+    table, lens = i32([[4, 2, 9, 1, 7, 3, 5, 8]]), i32([120])
+    call = lambda dst, keep=40: [x for c in ([ck.clone(), cv.clone(), w.clone()],)
+                                 for x in (*ops.evict_paged_kv(c[0], c[1], table, lens, c[2], keep, recent=8, dst_page_table=dst), *c)]
+    with pytest.raises(RuntimeError, match="must cover keep"):
+        call(table[:, :2])
+    want = call(None)
+    for dst in (table, table[:, :3]):
+        assert all(torch.equal(a, b) for a, b in zip(call(dst), want))

@@ -32,3 +32,16 @@ def test_scales_without_a_reciprocal(name):
         rows = _native.DecodeRows(q_heads=3)  # refused after the cache was found right
         message = error(lib.kvs_paged_decode_attention(C.byref(cache(dtype=2, **{name: scale})), C.byref(rows), None))
         assert ("reciprocal" in message) == refused and ("multiple of the KV heads" in message) != refused, (scale, message)
+
+
+def test_evict_destination_that_starts_where_the_table_does():
+    """The page table itself means in place. Other rows at its address are other tables, whose pages the
+    call would read and write at once. (One request's row may be cut short behind `keep`.)"""
+    lib, two = _native.load(), S2(512, 128)
+    rows = lambda **kw: _native.EvictRows(**dict(dict(keep=8, w_len=32, wo_len=32, weights=P16, weights_out=P16, weights_strides=two,
+                                                     weights_out_strides=two, dst_table=P16), **kw))
+    call = lambda c, **kw: error(lib.kvs_evict_paged(C.byref(c), C.byref(rows(**kw)), None))
+    assert "page_table itself" in call(cache(), dst_blocks=1)
+    assert "must cover keep" in call(cache(batch=1), dst_blocks=1, keep=17)
+    # taken as in place, then refused for their host addresses
+    assert "must be on device" in call(cache(), dst_blocks=2) and "must be on device" in call(cache(batch=1), dst_blocks=1)

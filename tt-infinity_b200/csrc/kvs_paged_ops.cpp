@@ -285,6 +285,10 @@ int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *r, void 
   const uint64_t cap = (uint64_t)cache->max_blocks * cache->block_size;
   CHECK(!r->dst_table || (uint64_t)r->dst_blocks * cache->block_size >= (r->keep < cap ? r->keep : cap),
         "%s: dst_page_table must cover keep (%u) slots", op, r->keep);
+  // the page table itself: in place
+  const bool in_place = !r->dst_table || r->dst_table == cache->page_table;
+  CHECK(!r->dst_table || !in_place || r->dst_blocks == cache->max_blocks || cache->batch == 1,
+        "%s: dst_page_table must be page_table itself or name fresh pages", op);
   CHECK(r->w_len >= cap && r->wo_len >= cap, "%s: weights must cover max_num_blocks_per_seq * block_size tokens", op);
   CHECK((uint64_t)cache->batch * cache->n_heads <= 0x7FFFFFFFull / 8, "%s: too many requests and heads", op);
   CHECK(r->weights != r->weights_out || (r->weights_strides[0] == r->weights_out_strides[0] &&
@@ -293,7 +297,7 @@ int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *r, void 
   Where w{op};
   TRY(add_cache(w, cache));
   TRY(w.add(r->seq_lens, "seq_lens"));
-  if (r->dst_table) TRY(w.add(r->dst_table, "dst_page_table"));
+  if (!in_place) TRY(w.add(r->dst_table, "dst_page_table"));
   TRY(w.add(r->weights, "weights"));
   TRY(w.add(r->weights_out, "weights_out"));
   TRY(w.add(r->kept, "kept"));
@@ -303,7 +307,7 @@ int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *r, void 
   TRY(sms_of(w.device, &sms, op));
   OnDevice on(w.device);
   p.seq_lens = r->seq_lens;
-  p.dst_table = r->dst_table;
+  p.dst_table = in_place ? nullptr : r->dst_table;
   p.dst_blocks = r->dst_blocks;
   p.weights = r->weights;
   p.weights_out = r->weights_out;

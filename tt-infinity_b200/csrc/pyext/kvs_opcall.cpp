@@ -315,14 +315,13 @@ PyObject *take_evict(PyObject *const *args, bool &called) {
     return not_taken();
   const at::Tensor kept = at::empty({batch, heads, keep}, lens->options()), fresh = at::empty({batch}, lens->options());
   kvs_evict_rows r{};
-  const bool in_place = !dst || dst->data_ptr() == static_cast<const void *>(cache.page_table);
-  r.seq_lens = ptr<int32_t>(lens), r.dst_table = in_place ? nullptr : ptr<int32_t>(dst);
+  r.seq_lens = ptr<int32_t>(lens), r.dst_table = ptr<int32_t>(dst);
   r.weights = ptr<float>(w), r.weights_out = ptr<float>(wo);
   strides(*w, 2, 1, r.weights_strides);
   strides(*wo, 2, 1, r.weights_out_strides);
   r.kept = static_cast<int32_t *>(kept.data_ptr()), r.new_lens = static_cast<int32_t *>(fresh.data_ptr());
   r.out_of_range = ptr<uint32_t>(count);
-  r.dst_blocks = in_place ? 0 : dst->size(1), r.w_len = w->size(2), r.wo_len = wo->size(2);
+  r.dst_blocks = dst ? dst->size(1) : 0, r.w_len = w->size(2), r.wo_len = wo->size(2);
   r.keep = keep, r.first = first, r.recent = recent;
   void *stream = c.stream();
   int rc;

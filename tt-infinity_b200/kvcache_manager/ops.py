@@ -541,11 +541,10 @@ def evict_paged_kv(cache_k: Any, cache_v: Any, page_table: Any, seq_lens: Any, w
     _check_counter(out_of_range)
     kept = torch.empty((batch, heads, keep), dtype=torch.int32, device=dev)
     new_lens = torch.empty((batch,), dtype=torch.int32, device=dev)
-    in_place = dst_page_table is None or dst_page_table.data_ptr() == page_table.data_ptr()
     rows = _native.EvictRows(
-        seq_lens.data_ptr(), None if in_place else dst_page_table.data_ptr(), weights.data_ptr(),
+        seq_lens.data_ptr(), _ptr(dst_page_table), weights.data_ptr(),
         weights_out.data_ptr(), _S2(*_strides(weights, 2, 1)), _S2(*_strides(weights_out, 2, 1)), kept.data_ptr(),
-        new_lens.data_ptr(), _ptr(out_of_range), 0 if in_place else dst_page_table.shape[1], weights.shape[2],
+        new_lens.data_ptr(), _ptr(out_of_range), 0 if dst_page_table is None else dst_page_table.shape[1], weights.shape[2],
         weights_out.shape[2], keep, first, recent)
     check(load().kvs_evict_paged(C.byref(cache), C.byref(rows), _stream(dev)))
     _changed(cache_k, cache_v, weights_out, out_of_range)
