@@ -215,3 +215,27 @@ def test_evict_destination_that_is_the_front_of_the_table(compiled, monkeypatch)
     want = call(None)
     for dst in (table, table[:, :3]):
         assert all(torch.equal(a, b) for a, b in zip(call(dst), want))
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_evict_destination_without_columns(compiled, monkeypatch):
+    """A given table that holds no slots is refused; it does not mean in place."""
+    if not compiled:
+        monkeypatch.setattr(_native, "opcall", False)
+    _, _, evict = decode_args()
+    before = evict["cache_k"].clone()
+    with pytest.raises(RuntimeError, match="must cover keep"):
+        ops.evict_paged_kv(**dict(evict, dst_page_table=torch.empty((2, 0), dtype=torch.int32, device="cuda")))
+    assert torch.equal(evict["cache_k"], before)
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_fill_positions_without_axes_of_any(compiled, monkeypatch):
+    """Given positions of no axis are refused; they do not mean the cache's positions."""
+    if not compiled:
+        monkeypatch.setattr(_native, "opcall", False)
+    fill, _, _ = decode_args()
+    before = fill["cache_k"].clone()
+    with pytest.raises(RuntimeError, match="positions must be"):
+        ops.qk_norm_rope_fill(**fill, positions=torch.empty((0, 2), dtype=torch.int32, device="cuda"))
+    assert torch.equal(fill["cache_k"], before)

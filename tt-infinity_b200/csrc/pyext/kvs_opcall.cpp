@@ -190,7 +190,7 @@ PyObject *take_fill(PyObject *const *args, bool &called) {
   if (cs->scalar_type() != at::kFloat || !cs->is_contiguous() || cs->size(0) > INT32_MAX || cs->size(1) > INT32_MAX) return not_taken();
   if (start->size(0) != cache.batch || cu->size(0) != (int64_t)cache.batch + 1) return not_taken();
   const int64_t n_axes = !positions ? 0 : positions->dim() == 2 ? positions->size(0) : 1;
-  if (positions && positions->size(positions->dim() - 1) != tokens) return not_taken();
+  if (positions && (positions->size(positions->dim() - 1) != tokens || n_axes < 1)) return not_taken();
   if (axes ? axes->size(0) * 2 != cs->size(1) : n_axes > 1) return not_taken();
   if (n_axes > 32 || (count && (count->scalar_type() != at::kInt || count->numel() < 1))) return not_taken();
   if (out && (out->sizes() != q->sizes() || out->scalar_type() != type)) return not_taken();
@@ -310,7 +310,7 @@ PyObject *take_evict(PyObject *const *args, bool &called) {
   if (!c.ok || first + recent > keep) return not_taken();
   if (!wo) wo = w;
   const int64_t batch = cache.batch, heads = cache.n_heads, cover = (int64_t)cache.max_blocks * cache.block_size;
-  if (lens->size(0) != batch || (dst && (dst->size(0) != batch || dst->size(1) > INT32_MAX)) || !sums_fit(*w, batch, heads, cover) ||
+  if (lens->size(0) != batch || (dst && (dst->size(0) != batch || dst->size(1) < 1 || dst->size(1) > INT32_MAX)) || !sums_fit(*w, batch, heads, cover) ||
       !sums_fit(*wo, batch, heads, cover) || (count && (count->scalar_type() != at::kInt || count->numel() < 1)))
     return not_taken();
   const at::Tensor kept = at::empty({batch, heads, keep}, lens->options()), fresh = at::empty({batch}, lens->options());

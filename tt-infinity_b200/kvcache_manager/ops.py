@@ -387,7 +387,7 @@ def qk_norm_rope_fill(q: Any, k: Any, v: Any, cos_sin: Any, cu_seqlens: Any, pag
     if positions is not None:
         n_axes = positions.shape[0] if positions.dim() == 2 else 1
         _int32(positions.dim(), positions=positions)
-        if positions.dim() not in (1, 2) or positions.shape[-1] != tokens:
+        if positions.dim() not in (1, 2) or positions.shape[-1] != tokens or n_axes < 1:
             raise RuntimeError("positions must be [tokens] or [n_axes, tokens]")
     if axes is not None and axes.shape[0] * 2 != cos_sin.shape[1]:
         raise RuntimeError("axes must hold rotary / 2 entries")
@@ -532,6 +532,8 @@ def evict_paged_kv(cache_k: Any, cache_v: Any, page_table: Any, seq_lens: Any, w
         raise RuntimeError(f"seq_lens size ({seq_lens.shape[0]}) must match batch_size ({batch})")
     if dst_page_table is not None and dst_page_table.shape[0] != batch:
         raise RuntimeError(f"dst_page_table must have batch_size ({batch}) rows")
+    if dst_page_table is not None and dst_page_table.shape[1] < 1:
+        raise RuntimeError(f"dst_page_table must cover keep ({keep}) slots")
     if keep <= 0 or keep >= 1 << 31 or first < 0 or recent < 0 or first + recent > keep:
         raise RuntimeError(f"keep ({keep}) must be 1 to 2^31 - 1, first ({first}) and recent ({recent}) not negative and "
                            "first + recent <= keep")
