@@ -45,3 +45,18 @@ def test_evict_destination_that_starts_where_the_table_does():
     assert "must cover keep" in call(cache(batch=1), dst_blocks=1, keep=17)
     # taken as in place, then refused for their host addresses
     assert "must be on device" in call(cache(), dst_blocks=2) and "must be on device" in call(cache(batch=1), dst_blocks=1)
+
+
+def test_attention_sums_that_overlap():
+    """weights_out may be weights itself, not other rows at its address; strides of a dimension of one
+    element do not matter."""
+    lib = _native.load()
+    rows = lambda **kw: _native.DecodeRows(**dict(dict(q=P16, out=P16, q_heads=4, scale=1.0, out_strides=S2(512, 128), weights=P16, weights_out=P16,
+                                                       w_len=32, weights_strides=S2(64, 32), weights_out_strides=S2(64, 32)), **kw))
+    attend = lambda c, **kw: error(lib.kvs_paged_decode_attention(C.byref(c), C.byref(rows(**kw)), None))
+    assert "not overlap" in attend(cache(), weights_strides=S2(32, 64)) and "not overlap" in attend(cache(), weights_strides=S2(64, 0))
+    assert "must be on device" in attend(cache()) and "must be on device" in attend(cache(), weights=2 * P16, weights_strides=S2(32, 64))
+    assert "must be on device" in attend(cache(batch=1), weights_strides=S2(0, 32))
+    ev = lambda c, s: error(lib.kvs_evict_paged(C.byref(c), C.byref(_native.EvictRows(
+        keep=8, w_len=32, wo_len=32, weights=P16, weights_out=P16, weights_strides=s, weights_out_strides=S2(64, 32))), None))
+    assert "not overlap" in ev(cache(), S2(32, 64)) and "must be on device" in ev(cache(batch=1), S2(0, 32))

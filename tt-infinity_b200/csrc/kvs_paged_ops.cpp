@@ -108,6 +108,12 @@ int check_cache(const kvs_paged_cache *c, const char *op, kvs::PagedCache *out) 
 
 // Dimensions of what a call writes: none of several elements may have stride 0 (a broadcast view).
 bool spread(const int64_t *strides, uint64_t n0, uint64_t n1) { return (n0 <= 1 || strides[0]) && (n1 <= 1 || strides[1]); }
+// A sum read and written at one address is read and written by the same strides.
+int check_sums(const kvs_paged_cache *c, const float *w, const int64_t *ws, const float *out, const int64_t *os, const char *op) {
+  CHECK(w != out || ((c->batch <= 1 || ws[0] == os[0]) && (c->n_heads <= 1 || ws[1] == os[1])),
+        "%s: weights_out must be weights itself or not overlap it", op);
+  return KVS_OK;
+}
 int check_written(const kvs_paged_cache *c, const char *op) {
   CHECK(spread(c->k_strides, c->num_blocks, c->n_heads) && spread(c->v_strides, c->num_blocks, c->n_heads) &&
             (c->block_size <= 1 || (c->k_strides[2] && c->v_strides[2])),
@@ -234,6 +240,7 @@ int kvs_paged_decode_attention(const kvs_paged_cache *cache, const kvs_decode_ro
   CHECK((r->weights == nullptr) == (r->weights_out == nullptr), "%s: weights and weights_out go together", op);
   CHECK(!r->weights || r->w_len >= (uint64_t)cache->max_blocks * cache->block_size,
         "%s: weights must cover max_num_blocks_per_seq * block_size tokens", op);
+  if (r->weights) TRY(check_sums(cache, r->weights, r->weights_strides, r->weights_out, r->weights_out_strides, op));
   CHECK((reinterpret_cast<uintptr_t>(r->workspace) & 255) == 0, "%s: workspace must be 256-byte aligned", op);
   Where w{op};
   TRY(add_cache(w, cache));
@@ -291,9 +298,7 @@ int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *r, void 
         "%s: dst_page_table must be page_table itself or name fresh pages", op);
   CHECK(r->w_len >= cap && r->wo_len >= cap, "%s: weights must cover max_num_blocks_per_seq * block_size tokens", op);
   CHECK((uint64_t)cache->batch * cache->n_heads <= 0x7FFFFFFFull / 8, "%s: too many requests and heads", op);
-  CHECK(r->weights != r->weights_out || (r->weights_strides[0] == r->weights_out_strides[0] &&
-                                         r->weights_strides[1] == r->weights_out_strides[1]),
-        "%s: weights_out must be weights itself or not overlap it", op);
+  TRY(check_sums(cache, r->weights, r->weights_strides, r->weights_out, r->weights_out_strides, op));
   Where w{op};
   TRY(add_cache(w, cache));
   TRY(w.add(r->seq_lens, "seq_lens"));
