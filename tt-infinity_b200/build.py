@@ -83,6 +83,8 @@ def build_opcall(force: bool = False) -> Path:
         import torch
     except ImportError:  # the operators take torch tensors: nothing to build for
         return out
+    if torch.version.cuda is None or not (Path(torch.__file__).parent / "lib" / "libc10_cuda.so").exists():
+        return out  # nor without torch's CUDA part
     deps = [OPCALL_SRC, ROOT / "include" / "kvs.h", Path(torch.__file__)]
     if not force and out.exists() and all(d.stat().st_mtime < out.stat().st_mtime for d in deps):
         return out
@@ -103,10 +105,15 @@ def build_opcall(force: bool = False) -> Path:
 
 
 def build(debug: bool = False, verbose: bool = False, force: bool = False) -> Path:
+    """The library first: it needs neither Python's nor torch's headers."""
+    if force or needs_build(OUT):
+        build_library(debug, verbose)
     build_fastcall(force)
     build_opcall(force)
-    if not force and not needs_build(OUT):
-        return OUT
+    return OUT
+
+
+def build_library(debug: bool = False, verbose: bool = False) -> None:
     flags = ARCH + [
         "-std=c++17",
         "--threads", "0",  # compile the sources side by side
@@ -128,7 +135,6 @@ def build(debug: bool = False, verbose: bool = False, force: bool = False) -> Pa
     if verbose:
         sys.stderr.write(res.stderr)
     os.replace(str(OUT) + ".tmp", OUT)
-    return OUT
 
 
 if __name__ == "__main__":
