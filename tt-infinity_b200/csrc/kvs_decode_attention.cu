@@ -32,8 +32,8 @@
 // further below a first token that takes most of the attention, so fp16 probabilities are held 2^15
 // times larger: half a step down to 2^-29 of the largest, 2^-40 of it below. (Rows of 512 tokens, the
 // first one 15 / 17 / 19 nats above the others, of value 0: fp16 outputs are off by half a step; unscaled
-// by 1.2 / 26 / 26 %. No time is lost to it.) An e4m3 cache is widened to
-// fp16, which holds every e4m3 value; the queries are scaled by a power of two per head to fit fp16.
+// by 1.2 / 26 / 26 %. No time is lost to it.) An e4m3 cache is widened to fp16, which holds every e4m3
+// value; the queries are scaled by a power of two per head to fit fp16.
 #include "kvs_paged_ops.cuh"
 
 #include <cuda_bf16.h>
@@ -59,9 +59,10 @@ enum Kind { kKindBf16, kKindFp16, kKindE4m3 };
 
 // How a kernel streams: tiles in a warp's ring, bytes of a CTA's rings and CTAs per SM, by bytes per
 // element, padded head_dim and column tiles of 8 heads. Rows of up to 128 bytes carry few bytes per
-// instruction, so they get more warps where registers allow: 3 CTAs per SM with 64 KiB each (e4m3, head_dim 128, 64 mixed contexts up to 12001 tokens:
-// 168 us against 171 us with 4 CTAs of 48 KiB and 172 us with 2 of 96 KiB). Longer rows take 2 CTAs of
-// 96 KiB, and rows of 512 bytes one of 192 KiB, three tiles per warp being the least that keeps loads
+// instruction, so they get more warps where registers allow: 3 CTAs per SM with 64 KiB each (e4m3,
+// head_dim 128, 64 mixed contexts up to 12001 tokens: 168 us against 171 us with 4 CTAs of 48 KiB and
+// 172 us with 2 of 96 KiB). Longer rows take 2 CTAs of 96 KiB, and rows of 512 bytes one of 192 KiB,
+// three tiles per warp being the least that keeps loads
 // in flight while a tile is worked on.
 struct Shape {
   int stages, ring, ctas;
@@ -806,8 +807,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
 }
 
 // Joins the partials of a (request, head tile): slot 1 of the CTA that took its first units, then slot 0
-// of the CTAs after it. Blocks stand for CTAs or, where there are fewer, for (request, head tile)s. A piece is 16 elements of 8 heads (one fragment); a block takes
-// p.pieces of them, each by 8 / p.pieces warps that take every so many partials and add up in order.
+// of the CTAs after it. Blocks stand for CTAs or, where there are fewer, for (request, head tile)s. A
+// piece is 16 elements of 8 heads (one fragment); a block takes p.pieces of them, each by 8 / p.pieces
+// warps that take every so many partials and add up in order.
 template <int DP, int NT, bool k8>
 __device__ __forceinline__ void join_part(const KernelParams &p, uint32_t block) {
   constexpr int kSteps = DP / 16;
@@ -908,8 +910,8 @@ __device__ __forceinline__ void join_part(const KernelParams &p, uint32_t block)
 }
 
 // weights_out[b, h, t] = weights[b, h, t] + sum over the heads of the group of 2^(score - lse), for
-// p.weight_chunk tokens. The log-sum-exp of a head that was split is found from its parts here, a warp per head, so
-// that this needs no wait for the join.
+// p.weight_chunk tokens. The log-sum-exp of a head that was split is found from its parts here, a warp per
+// head, so that this needs no wait for the join.
 constexpr uint32_t kWeightTokens = 1024;  // tokens a block looks at at once
 template <int NT>
 __device__ __forceinline__ void add_weights(const KernelParams &p, uint32_t block) {

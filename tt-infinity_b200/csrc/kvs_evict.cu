@@ -45,7 +45,7 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   if (w != w) return 0xFFC00000u;
   if (w == 0.f) w = 0.f;  // one zero
   const uint32_t u = __float_as_uint(w);
-  return u == 0x80000000u ? 0x80000000u : (u & 0x80000000u ? ~u : u | 0x80000000u);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
 __device__ __forceinline__ uint32_t length_of(const EvictParams &p, uint32_t b) {

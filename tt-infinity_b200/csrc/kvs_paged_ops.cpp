@@ -186,6 +186,8 @@ int kvs_qk_norm_rope_fill(const kvs_paged_cache *cache, const kvs_qkv_rows *r, v
   if (r->q_weight) TRY(w.add(r->q_weight, "q_weight"));
   if (r->k_weight) TRY(w.add(r->k_weight, "k_weight"));
   if (r->out_of_range) TRY(w.add(r->out_of_range, "out_of_range"));
+  int sms = 0;
+  TRY(sms_of(w.device, &sms, op));
   OnDevice on(w.device);
   p.q = static_cast<const uint8_t *>(r->q);
   p.k = static_cast<const uint8_t *>(r->k);
@@ -213,7 +215,7 @@ int kvs_qk_norm_rope_fill(const kvs_paged_cache *cache, const kvs_qkv_rows *r, v
   p.interleaved = r->interleaved;
   p.zero_rest = r->zero_rest;
   p.page = kvs::Divisor(p.c.block_size);
-  CUDA_TRY(kvs::launch_qkv_fill(p, static_cast<cudaStream_t>(stream)), op);
+  CUDA_TRY(kvs::launch_qkv_fill(p, sms, static_cast<cudaStream_t>(stream)), op);
   return KVS_OK;
 }
 
@@ -318,8 +320,6 @@ int kvs_evict_paged(const kvs_paged_cache *cache, const kvs_evict_rows *r, void 
   p.weights_out = r->weights_out;
   p.w_req = r->weights_strides[0], p.w_head = r->weights_strides[1];
   p.wo_req = r->weights_out_strides[0], p.wo_head = r->weights_out_strides[1];
-  p.w_len = r->w_len;
-  p.wo_len = r->wo_len;
   p.keep = r->keep;
   p.first = r->first;
   p.recent = r->recent;

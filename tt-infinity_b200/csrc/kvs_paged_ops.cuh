@@ -73,7 +73,7 @@ struct QkvFillParams {
   int interleaved, zero_rest;
   Divisor page;                 // block_size
 };
-cudaError_t launch_qkv_fill(const QkvFillParams &p, cudaStream_t stream);
+cudaError_t launch_qkv_fill(const QkvFillParams &p, int sms, cudaStream_t stream);
 
 struct DecodeAttentionParams {
   PagedCache c;
@@ -103,7 +103,6 @@ struct EvictParams {
   const float *weights;
   float *weights_out;
   int64_t w_req, w_head, wo_req, wo_head;
-  uint32_t w_len, wo_len;
   uint32_t keep, first, recent;
   int32_t *kept;              // [batch][n_heads][keep]
   int32_t *new_lens;          // [batch]

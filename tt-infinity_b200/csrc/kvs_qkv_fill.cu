@@ -333,13 +333,13 @@ __global__ void __launch_bounds__(32) qkv_fill_kernel(const __grid_constant__ Qk
 }
 
 template <bool kBf, bool kInter, int PP, int kLanes>
-cudaError_t run(const QkvFillParams &p, cudaStream_t stream) {
+cudaError_t run(const QkvFillParams &p, int sms, cudaStream_t stream) {
   using R = Rows<kBf, kInter, PP, kLanes>;
-  // Rows per warp: many share one lookup and one set of coefficients, as long as enough warps are left.
+  // Rows per warp: many share one lookup and one set of coefficients, as long as 16 warps per SM are left.
   // 8192 tokens of 64 + 2 x 8 heads: 57 us with up to 64 rows per warp, 63 us with 16.
   const uint32_t steps = (p.q_heads + R::step - 1) / R::step;
   uint32_t per = 8;
-  while (per > 1 && (uint64_t)p.tokens * ((steps + per - 1) / per) < 148 * 16) per /= 2;
+  while (per > 1 && (uint64_t)p.tokens * ((steps + per - 1) / per) < 16ull * sms) per /= 2;
   const uint32_t q_parts = (steps + per - 1) / per, kv_parts = (p.c.n_heads + per * R::step - 1) / (per * R::step);
   const dim3 grid(p.tokens, q_parts + kv_parts);
   if (grid.y > 65535) return cudaErrorInvalidValue;
@@ -354,25 +354,25 @@ cudaError_t run(const QkvFillParams &p, cudaStream_t stream) {
 }
 
 template <bool kBf, bool kInter>
-cudaError_t run_dim(const QkvFillParams &p, cudaStream_t stream) {
+cudaError_t run_dim(const QkvFillParams &p, int sms, cudaStream_t stream) {
   const uint32_t d = p.c.head_dim;
   // 16-byte halves where both the rotated part and the rest split into eights of pairs
   if (p.rotary % 16 == 0 && d % 16 == 0) {
-    if (d <= 64) return run<kBf, kInter, 8, 4>(p, stream);
-    if (d <= 128) return run<kBf, kInter, 8, 8>(p, stream);
-    return run<kBf, kInter, 8, 16>(p, stream);
+    if (d <= 64) return run<kBf, kInter, 8, 4>(p, sms, stream);
+    if (d <= 128) return run<kBf, kInter, 8, 8>(p, sms, stream);
+    return run<kBf, kInter, 8, 16>(p, sms, stream);
   }
-  if (d <= 64) return run<kBf, kInter, 4, 8>(p, stream);
-  if (d <= 128) return run<kBf, kInter, 4, 16>(p, stream);
-  return run<kBf, kInter, 4, 32>(p, stream);
+  if (d <= 64) return run<kBf, kInter, 4, 8>(p, sms, stream);
+  if (d <= 128) return run<kBf, kInter, 4, 16>(p, sms, stream);
+  return run<kBf, kInter, 4, 32>(p, sms, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_qkv_fill(const QkvFillParams &p, cudaStream_t stream) {
+cudaError_t launch_qkv_fill(const QkvFillParams &p, int sms, cudaStream_t stream) {
   if (p.tokens == 0) return cudaSuccess;
-  if (p.interleaved) return p.dtype == kBf16 ? run_dim<true, true>(p, stream) : run_dim<false, true>(p, stream);
-  return p.dtype == kBf16 ? run_dim<true, false>(p, stream) : run_dim<false, false>(p, stream);
+  if (p.interleaved) return p.dtype == kBf16 ? run_dim<true, true>(p, sms, stream) : run_dim<false, true>(p, sms, stream);
+  return p.dtype == kBf16 ? run_dim<true, false>(p, sms, stream) : run_dim<false, false>(p, sms, stream);
 }
 
 }  // namespace kvs

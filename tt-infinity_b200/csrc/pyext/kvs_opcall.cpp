@@ -38,7 +38,6 @@ struct Call {
   bool ok = true, grad = c10::GradMode::is_enabled();
 
   const at::Tensor *tensor(int i, int64_t dims, bool optional = false) {
-    static const at::Tensor none;
     PyObject *o = args[i];
     if (o == Py_None && optional) return nullptr;
     if (!THPVariable_CheckExact(o)) return fail();
