@@ -53,7 +53,8 @@ constexpr int kThreads = 32 * kWarps;
 constexpr uint32_t kTile = 16;  // tokens per warp tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kLift = 15.f;  // fp16 probabilities are 2^kLift times as large: at most 2^15 < 65504
+// fp16 probabilities are 2^kLift times as large: at most 2^15 < 65504
+constexpr float kLift = 15.f, kUnlift = 1.f / 32768.f;
 
 enum Kind { kKindBf16, kKindFp16, kKindE4m3 };
 
@@ -283,7 +284,6 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
   constexpr bool kBf = kKind == kKindBf16;
   constexpr bool k8 = kKind == kKindE4m3;
   constexpr int kSteps = DP / 16;
-  constexpr float lift = kBf ? 0.f : kLift, unlift = kBf ? 1.f : 1.f / 32768.f;  // 2^-lift
   extern __shared__ uint8_t smem_raw[];
   uint8_t *const smem = smem_raw + (-smem_addr(smem_raw) & 511);
   __shared__ uint64_t s_scan[kWarps];
@@ -659,7 +659,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
       uint32_t pb[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float base0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0] - lift, base1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1] - lift;
+        float base0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], base1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+        if constexpr (!kBf) base0 -= kLift, base1 -= kLift;
         const float e0 = exp2_fast(sc[nt][0] - base0), e1 = exp2_fast(sc[nt][1] - base1);
         const float e2 = exp2_fast(sc[nt][2] - base0), e3 = exp2_fast(sc[nt][3] - base1);
         l[nt][0] += e0 + e2;
@@ -702,12 +703,13 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kKind, DP, NT>::ctas)) decode_a
         l[nt][i] += __shfl_xor_sync(~0u, l[nt][i], 4);
         l[nt][i] += __shfl_xor_sync(~0u, l[nt][i], 8);
         l[nt][i] += __shfl_xor_sync(~0u, l[nt][i], 16);
-        if (kBf) continue;
-        l[nt][i] *= unlift;  // exact: what follows knows nothing of the lift
+        if constexpr (!kBf) {
+          l[nt][i] *= kUnlift;  // exact: what follows knows nothing of the lift
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          acc[nt][s][i] *= unlift;
-          acc[nt][s][2 + i] *= unlift;
+          for (int s = 0; s < kSteps; ++s) {
+            acc[nt][s][i] *= kUnlift;
+            acc[nt][s][2 + i] *= kUnlift;
+          }
         }
       }
 
