@@ -337,14 +337,16 @@ int kvs_paged_fill_varlen_layers(uint32_t n_layers, const void *const *k_fills, 
  *
  * kvs_paged_cache describes one layer's cache: row (block, head, slot) of K is head_dim contiguous
  * elements at k + block * k_strides[0] + head * k_strides[1] + slot * k_strides[2] (bytes, multiples
- * of 16, not negative; the address a multiple of 16; V likewise), which covers [num_blocks, heads, block_size, head_dim] and
- * vLLM's [num_blocks, block_size, heads, head_dim]. page_table: [batch][max_blocks] int32; entries
- * <= 0 hold nothing, entries >= num_blocks are out of range, and tokens in either take no part. An
- * e4m3 cache holds value / k_scale and value / v_scale, saturated; other types use scales of 1. A scale
- * is positive and finite, and so is its reciprocal.
- * head_dim: a multiple of 8 (16 for e4m3) up to 256. Rows behind a request's length, and all that a
- * masked slot holds, are not read. All arrays are device memory of one GPU; calls are asynchronous
- * on `stream`, make no allocation and keep no state, so they can be captured into CUDA graphs. */
+ * of 16, not negative; the address a multiple of 16; V likewise), which covers [num_blocks, heads,
+ * block_size, head_dim] and vLLM's [num_blocks, block_size, heads, head_dim]. page_table:
+ * [batch][max_blocks] int32; entries <= 0 hold nothing, entries >= num_blocks are out of range, and
+ * tokens in either take no part. An e4m3 cache holds value / k_scale and value / v_scale, saturated;
+ * other types use scales of 1. A scale is positive and finite, and so is its reciprocal. head_dim: a
+ * multiple of 8 (16 for e4m3) up to 256. Limits: 65535 requests and KV heads, 2^31 - 1 blocks, as many
+ * tokens in a row of the page table; 65535 query heads in a fill, 1024 for each KV head in an attention.
+ * Rows behind a request's length, and all that a masked slot holds, are not read. All arrays are device
+ * memory of one GPU; calls are asynchronous on `stream`, make no allocation and keep no state, so they
+ * can be captured into CUDA graphs. */
 #define KVS_DTYPE_BF16 0
 #define KVS_DTYPE_FP16 1
 #define KVS_DTYPE_E4M3 2
@@ -394,11 +396,13 @@ int kvs_qk_norm_rope_fill(const kvs_paged_cache *cache, const kvs_qkv_rows *rows
  * by max_blocks * block_size: out = sum softmax(scale * q . k) v. A row with no token gives zeros and
  * a log-sum-exp of -infinity. lse: optional [batch][q_heads] fp32, natural logarithm. weights_out
  * (optional, [batch][n_heads][w_len] fp32, strides in elements between requests and heads; `weights`
- * itself, or apart from it): weights_out[b][h][t] = weights[b][h][t] + the softmax weights of token t summed over the
- * query heads of h, for t < seq_lens[b]; w_len must cover max_blocks * block_size. The order of every
- * sum is fixed by the lengths, so equal calls give equal bits. workspace: at least
+ * itself, or apart from it): weights_out[b][h][t] = weights[b][h][t] + the softmax weights of token t
+ * summed over the query heads of h, for t < seq_lens[b]; w_len must cover max_blocks * block_size. The
+ * order of every sum is fixed by the lengths, so equal calls give equal bits. workspace: at least
  * kvs_decode_attention_workspace bytes, 256-byte aligned, its contents of no matter; concurrent
- * calls need one each. */
+ * calls need one each. With weights it holds 4 * batch * q_heads * max_blocks * block_size bytes of
+ * scores (64 requests, 64 query heads, rows of 131072 tokens: 2 GiB), whatever the lengths are: a call
+ * whose contexts are short is given a page table (and weights) cut to the longest one. */
 typedef struct {
   const void *q;
   void *out;
@@ -419,16 +423,18 @@ int kvs_decode_attention_workspace(const kvs_paged_cache *cache, const kvs_decod
 int kvs_paged_decode_attention(const kvs_paged_cache *cache, const kvs_decode_rows *rows, void *stream);
 
 /* Eviction by accumulated attention weight. Per request and KV head, of the tokens below
- * seq_lens[b] that have a page: positions < first and >= seq_lens[b] - recent stay, and of the others
- * those of the largest weight (equal weights: the lowest position; NaN counts as the largest), keep
- * in all (first + recent <= keep). kept: [batch][n_heads][keep] int32, the kept positions in order,
- * then -1; new_lens: [batch] int32, min(keep, tokens). Kept rows of K and V move to slots 0, 1, ... of
+ * seq_lens[b] (bounded by max_blocks * block_size) that have a page: positions < first and
+ * >= seq_lens[b] - recent stay, and of the others those of the largest weight (equal weights: the lowest
+ * position; NaN counts as the largest), keep in all (first + recent <= keep). kept:
+ * [batch][n_heads][keep] int32, the kept positions in order, then -1; new_lens: [batch] int32,
+ * min(keep, tokens). Kept rows of K and V move to slots 0, 1, ... of
  * dst_table ([batch][dst_blocks] int32, covering keep slots; its blocks must be in no other table row
  * of the call), or, where dst_table is null or the page table itself, of the request's own blocks, in
- * place (then shared by no other request). A slot without a valid block stores nothing and increments *out_of_range when
- * given. weights: [batch][n_heads][w_len] fp32 (strides in elements between requests and heads), w_len
- * covering max_blocks * block_size; weights_out (`weights` itself, or apart from it) receives the kept tokens' weights,
- * then zeros up to seq_lens[b]. cache->dtype gives the element size only: rows are moved as they are. */
+ * place (then shared by no other request and named once). A slot without a valid block stores nothing and increments
+ * *out_of_range when given. weights: [batch][n_heads][w_len] fp32 (strides in elements between requests
+ * and heads), w_len covering max_blocks * block_size; weights_out (`weights` itself, or apart from it)
+ * receives the kept tokens' weights, then zeros up to seq_lens[b]. cache->dtype gives the element size
+ * only: rows are moved as they are. */
 typedef struct {
   const int32_t *seq_lens, *dst_table;
   const float *weights;

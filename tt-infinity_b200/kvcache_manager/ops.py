@@ -436,8 +436,10 @@ def paged_decode_attention(q: Any, cache_k: Any, cache_v: Any, page_table: Any, 
 
     weights (fp32 [batch, num_kv_heads, tokens], covering the page table's tokens) accumulates what
     evict_paged_kv chooses by: weights_out (default: weights itself) becomes weights plus each token's
-    softmax weight summed over the KV head's query heads, for the tokens below seq_lens. Equal calls
-    give equal bits. Asynchronous on the current stream; no backward pass."""
+    softmax weight summed over the KV head's query heads, for the tokens below seq_lens. Such a call
+    allocates 4 bytes for each query head and token of the page table (64 requests, 64 query heads and rows
+    of 131072 tokens: 2 GiB), whatever the lengths are: cut page_table and weights to the longest context.
+    Equal calls give equal bits. Asynchronous on the current stream; no backward pass."""
     fast = _native.opcall if _native.opcall is not None else _native.load_opcall()
     if fast:
         done = fast.attend(q, cache_k, cache_v, page_table, seq_lens, scale, window, k_scale, v_scale, out, return_lse,
@@ -507,7 +509,7 @@ def evict_paged_kv(cache_k: Any, cache_v: Any, page_table: Any, seq_lens: Any, w
     The kept rows move in order to slots 0, 1, ... of dst_page_table (int32 [batch, blocks], covering
     keep slots), fresh pages that no table of the call reads, so pages shared between requests or held
     by a store stay as they are. Without dst_page_table (or with page_table itself) they move within the
-    request's own pages, which then no other request may share. A slot without a valid page stores
+    request's own pages, which then no other request may share, nor name one page twice. A slot without a valid page stores
     nothing and is counted in out_of_range (int32, one element). weights: fp32 [batch, num_kv_heads,
     tokens] as paged_decode_attention accumulates them, covering the page table's tokens; weights_out
     (default: weights itself) receives the kept tokens' weights, then zeros up to seq_lens. Keys keep the
